@@ -15,7 +15,7 @@ _lib = None
 
 _i64, _i32, _f32, _u64, _vp, _sz = C.c_int64, C.c_int, C.c_float, C.c_uint64, C.c_void_p, C.c_size_t
 
-ABI_VERSION = 10     # include/gsdf_hip.h: GSDF_ABI_VERSION this binding was written against
+ABI_VERSION = 11     # include/gsdf_hip.h: GSDF_ABI_VERSION this binding was written against
 
 
 class RasterInstr(C.Structure):
@@ -120,6 +120,15 @@ _SIGS = {
     "gsdf_adam_step_zero_grad": (C.c_int, [_i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _i64, _vp]),
     "gsdf_knn_ws_bytes": (_sz, [_i64]),
     "gsdf_knn_mean_dist2": (C.c_int, [_i64] + [_vp] * 4),
+    "gsdf_dropout": (C.c_int, [_i64, _i64, _i32, _vp, _i64, _vp, _i64, C.c_double, _u64, _u64, _vp, _vp, _i64, _vp]),
+    "gsdf_lowrank_save_bytes": (_sz, [_vp]),
+    "gsdf_lowrank_fwd_ws_bytes": (_sz, [_vp]),
+    "gsdf_lowrank_bwd_ws_bytes": (_sz, [_vp]),
+    "gsdf_lowrank_fwd": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "gsdf_lowrank_bwd": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "gsdf_router_balance_ws_bytes": (_sz, [_i64, _i32]),
+    "gsdf_router_balance_fwd": (C.c_int, [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _i32] + [_vp] * 6),
+    "gsdf_router_balance_bwd": (C.c_int, [_i64, _i32, _i32, _vp, _i64] + [_vp] * 5),
 }
 
 
@@ -185,6 +194,13 @@ class RaySamplerArgs(C.Structure):
                 ("free_sample_num", C.c_int), ("surface_sample_num", C.c_int), ("map_origin", C.c_float * 3), ("map_size_inv", C.c_float),
                 ("map_half", C.c_float), ("range_lo", C.c_float * 3), ("range_hi", C.c_float * 3), ("sample_std", C.c_float),
                 ("truncated_dis", C.c_float)]
+
+
+class LowrankArgs(C.Structure):
+    """include/gsdf_hip.h: gsdf_lowrank_args"""
+    _fields_ = [("rows", C.c_int64), ("x_stride", C.c_int64), ("n_in", C.c_int), ("n_out", C.c_int), ("rank", C.c_int), ("n_adapters", C.c_int),
+                ("dtype", C.c_int), ("ids_64", C.c_int), ("x", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p), ("ids", C.c_void_p),
+                ("scales", C.c_void_p), ("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64), ("offset_dev", C.c_void_p)]
 
 
 _words = {}          # (thread id, device index) -> HostWords: two threads never arm the same word, one word per device

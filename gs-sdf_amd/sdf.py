@@ -448,10 +448,15 @@ class TCNNNetwork:
         # gradients are accumulated IN PLACE, and a stream for that half of the backward (see _MlpFn.backward)
         self.grad_sinks, self.aux_stream = None, None
 
-    def forward(self, x):
+    def forward(self, x, adapters=None, ids=None):
+        """`adapters`, `ids` (not in the reference's interface): low-rank adapters (adapters.LowRankAdapters, n_in -> n_out of this network) beside the
+        shared network, row i takes adapter ids[i] (outside [0, n_adapters): none) — one decoder for the points of many maps."""
         if x.dim() != 2 or x.shape[1] != self.dims[0]:
             raise RuntimeError(f"TCNNNetwork.forward: expected [B,{self.dims[0]}]")
-        return _MlpFn.apply(x, self.params_, self.biases_, tuple(self.dims), self.grad_sinks, self.aux_stream)
+        if (adapters is None) != (ids is None):
+            raise RuntimeError("TCNNNetwork.forward: adapters and ids go together")
+        out = _MlpFn.apply(x, self.params_, self.biases_, tuple(self.dims), self.grad_sinks, self.aux_stream)
+        return out if adapters is None else adapters(x, ids, base=out)
 
     __call__ = forward
 

@@ -40,7 +40,7 @@ const char *gsdf_last_error(void);
 /* ABI version; bumped on any signature change.  Every binding compares gsdf_abi_version() of the library it loaded with the
  * GSDF_ABI_VERSION of the header it was written against and refuses to run on a mismatch (gs_sdf_amd/capi.py: lib(); the C++
  * operator layer: gsplat_ops.cpp static initialiser): a stale libgsdf_hip.so fails at load, not on the device. */
-#define GSDF_ABI_VERSION 10
+#define GSDF_ABI_VERSION 11
 int gsdf_abi_version(void);
 
 /* Deterministic mode (process-wide — a step's backward kernels are launched by the autograd engine's thread, not by the caller's; on != 0 switches
@@ -685,6 +685,61 @@ int gsdf_normal_consistency_bwd(int height, int width, const float *intrinsics4_
 int gsdf_normal_consistency_fwd_bwd(int height, int width, const float *intrinsics4_host, const float *pose_c2w_host,
                                     const float *depth, const float *alpha, const float *render_normal, const float *v_loss,
                                     float *loss, float *v_depth, float *v_render_normal, gsdf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * L1-L3  one decoder for many maps (no reference counterpart: the reference trains one network per map): low-rank adapters that
+ *        differ row by row beside a shared projection, dropout on their input, the balance loss of the router that chooses them.
+ * Element types: GSDF_F32, GSDF_F16, GSDF_BF16 (one type for all element pointers of a call); sums are held in 32 bits, a result is rounded once.
+ * Rows may start at any element: strides are in elements, a row's elements are neighbours, no alignment beyond the element's is asked for.
+ * Results do not depend on the order in which workgroups run (with or without gsdf_deterministic).
+ * ---------------------------------------------------------------------------------------- */
+#define GSDF_F32 0
+#define GSDF_F16 1
+#define GSDF_BF16 2
+
+/* L2  y = [residual +] drop(x) on a [rows, cols] matrix.  The mask comes from Philox4x32-10 and is never stored: element (row, col) looks at 16 bits
+ * of the block with the counter (col / 8, row, offset mod 2^32, offset / 2^32) and the key (seed mod 2^32, seed / 2^32): bits [16 (col % 2), +16) of word
+ * (col % 8) / 2.  Dropped (exactly 0, whatever x holds) where they are below round(65536 p); what stays is multiplied by 65536 / (65536 - round(65536 p)).
+ * The backward pass is the same call on the upstream gradient with residual = NULL.  offset_dev (may be NULL): a device word added to `offset` when the
+ * kernel runs, so that every replay of a captured graph can have a mask of its own.  rows < 2^32, cols < 2^33; y may be x or residual. */
+int gsdf_dropout(int64_t rows, int64_t cols, int dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, double p,
+                 uint64_t seed, uint64_t offset, const uint64_t *offset_dev, void *y, int64_t y_stride, gsdf_stream_t stream);
+
+/* L1  y_t = base_t + s_g B_g A_g drop(x_t) with the adapter g = ids[t] of row t; a row whose id is outside [0, n_adapters) has none and keeps base_t.
+ * x [rows, n_in], a [n_adapters, rank, n_in], b [n_adapters, n_out, rank] (contiguous), ids [rows] int32 (ids_64 = 0) or int64, scales [n_adapters] fp32
+ * (NULL: 1), base / y [rows, n_out] (base NULL: 0; y may be base).  Dropout as in gsdf_dropout on the matrix x (p = 0: none).
+ * fwd: save (gsdf_lowrank_save_bytes) is written for the backward pass, NULL where none follows; ws: gsdf_lowrank_fwd_ws_bytes.
+ * bwd: dx [rows, n_in], da, db (any may be NULL) are overwritten, an adapter without rows gets zeros, a row without an adapter dx = 0; dbase = dy is the
+ *      caller's.  args, x, ids, a, b and *offset_dev as in the forward call; ws: gsdf_lowrank_bwd_ws_bytes. */
+#define GSDF_LOWRANK_MAX_RANK 128
+#define GSDF_LOWRANK_MAX_ADAPTERS 1024
+typedef struct {
+  int64_t rows, x_stride;
+  int n_in, n_out, rank, n_adapters, dtype, ids_64;
+  const void *x, *a, *b, *ids;
+  const float *scales;
+  double p;
+  uint64_t seed, offset;
+  const uint64_t *offset_dev;
+} gsdf_lowrank_args;
+size_t gsdf_lowrank_save_bytes(const gsdf_lowrank_args *args);
+size_t gsdf_lowrank_fwd_ws_bytes(const gsdf_lowrank_args *args);
+size_t gsdf_lowrank_bwd_ws_bytes(const gsdf_lowrank_args *args);
+int gsdf_lowrank_fwd(const gsdf_lowrank_args *args, const void *base, int64_t base_stride, void *y, int64_t y_stride, void *save, void *ws,
+                     gsdf_stream_t stream);
+int gsdf_lowrank_bwd(const gsdf_lowrank_args *args, const void *dy, int64_t dy_stride, const void *save, void *dx, int64_t dx_stride, void *da, void *db,
+                     void *ws, gsdf_stream_t stream);
+
+/* L3  balance loss of a router: with p = softmax(logits) [rows, n_experts], V the rows whose mask byte is not 0 (mask NULL: all), ids [rows, k] the experts
+ * each row went to (contiguous; ids outside [0, n_experts) count for nobody), counts[e] = their number in valid rows:
+ *     loss = n_experts * sum_e (counts[e] / (k V)) (sum_valid p_te / V),       0 where V is 0.
+ * fwd writes loss[1], counts[n_experts] and pull[n_experts] (for the backward pass); bwd writes v_logits [rows, n_experts] (contiguous) = v_loss[0] * dloss /
+ * dlogits, 0 in rows that are not valid (whose logits may hold anything).  counts are constants of the gradient.  A row of -inf alone has p = 0. */
+size_t gsdf_router_balance_ws_bytes(int64_t rows, int n_experts);
+int gsdf_router_balance_fwd(int64_t rows, int n_experts, int k, int dtype, const void *logits, int64_t stride, const void *ids, int ids_64,
+                            const uint8_t *mask, float *loss, int64_t *counts, float *pull, void *ws, gsdf_stream_t stream);
+int gsdf_router_balance_bwd(int64_t rows, int n_experts, int dtype, const void *logits, int64_t stride, const uint8_t *mask, const float *pull,
+                            const float *v_loss, void *v_logits, gsdf_stream_t stream);
 
 #ifdef __cplusplus
 }
