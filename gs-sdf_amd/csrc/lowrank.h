@@ -1,0 +1,92 @@
+// lowrank.h — what lowrank.hip (the plan, the C entries) and lowrank_kernels.h (the products, compiled once for each element type) share.
+#pragma once
+#include "adapter_common.h"
+
+namespace gsdf {
+
+static constexpr int LR_CUS = 256;          // compute units the ranges are dealt to
+static constexpr int LR_AIM = 40;           // rows of a range that are aimed at, at most
+static constexpr int LR_RANGE = 48;         // most rows of a range: three matrix tiles
+static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
+
+// ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------
+// All in one int32 buffer.  Group n_adapters holds the rows without an adapter.
+struct Plan {
+  int *order;      // [rows]: the row at each place, adapters one behind the other, rows of one adapter in their own order
+  int4 *range;     // [n_ranges]: adapter, first place, rows (0: unused), -
+  int4 *chunk;     // [max_chunks]: adapter, first place, rows (0: unused), slot of its partial sums (-1: the adapter's only chunk)
+  int2 *slots;     // [n_adapters]: first slot, chunks
+  int *hist;       // [blocks][n_adapters]: rows of each adapter in each workgroup's share
+  int rows, n_adapters, blocks, block_rows;
+  int per, wanted, n_ranges, max_chunks;
+};
+// Every range costs a compute unit about the bytes of its rows and of its adapter's weights, and ends with its adapter: `per` is the smallest size from
+// this one on that makes no more ranges than a multiple of the units (264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 take 20: 8192 rows of 8 KB).
+// `least`: rows that share the weights at least.
+static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int least) {
+  p->rows = (int)rows; p->n_adapters = n_adapters;
+  p->block_rows = rows <= LR_CUS * 1024 ? 1024 : (int)align_up((size_t)ceil_div(rows, LR_CUS), 1024);
+  p->blocks = (int)ceil_div(rows > 0 ? rows : 1, p->block_rows);
+  const int64_t waves = ceil_div(rows > 0 ? rows : 1, LR_CUS * LR_AIM);
+  p->wanted = (int)(LR_CUS * waves);
+  p->per = (int)ceil_div(rows > 0 ? rows : 1, p->wanted);
+  if (p->per < least) p->per = least;
+  const int64_t most = rows / LR_RANGE + n_adapters + 1;
+  p->n_ranges = (int)(p->wanted > most ? p->wanted : most);
+  p->max_chunks = (int)(rows / LR_CHUNK + n_adapters);
+  char *at = (char *)mem;
+  auto take = [&](size_t bytes) { char *r = at; at += align_up(bytes, 16); return r; };
+  p->range = (int4 *)take((size_t)p->n_ranges * 16);
+  p->chunk = (int4 *)take((size_t)p->max_chunks * 16);
+  p->slots = (int2 *)take((size_t)n_adapters * 8);
+  p->hist = (int *)take((size_t)p->blocks * n_adapters * 4);
+  p->order = (int *)take((size_t)rows * 4);
+  return (size_t)(at - (char *)mem);
+}
+// slots for the chunks of adapters with more than one: such an adapter has more than LR_CHUNK rows, so there are at most twice rows / LR_CHUNK of them
+static int64_t plan_max_slots(int64_t rows, int n_adapters) {
+  const int64_t twice = 2 * (rows / LR_CHUNK) + 1, all = rows / LR_CHUNK + n_adapters;
+  return rows <= LR_CHUNK ? 0 : (twice < all ? twice : all);
+}
+
+struct Ids {
+  const void *p;
+  int is_64, n_adapters;
+};
+__device__ __forceinline__ int group_of(Ids ids, int64_t row) {
+  const int64_t g = load_id(ids.p, ids.is_64, row);
+  return g >= 0 && g < ids.n_adapters ? (int)g : ids.n_adapters;
+}
+
+// ---- weights turned for the backward pass: A [g][r][k] -> [g][k][RP] (zeros behind the rank), B [g][n][r] -> [g][r][n] ----------------------
+// They go with the launch that begins the plan, which leaves the rest of the card idle.
+struct TurnArgs {
+  const void *in[2];
+  void *out[2];
+  int rows[2], cols[2], out_ld[2];      // of one adapter's matrix, and of the turned one
+  int blocks0, blocks;                  // tiles of 64 x 64 of the first matrix, of both
+  int es;
+};
+// a call, with everything in its place
+struct Lowrank {
+  gsdf_lowrank_args a;
+  Dropout drop;
+  Plan plan;
+  int rt, rp, es;
+  int64_t ht_ld;
+  // saved by the forward pass (beside the plan)
+  float *ht;
+  void *turned[2];
+  // workspace
+  float *h, *dh, *dht, *part[2];
+  size_t save_bytes, fwd_ws_bytes, bwd_ws_bytes;
+};
+
+void lowrank_plan_launch(const Plan &p, const Ids &ids, const TurnArgs &turn, hipStream_t stream);
+TurnArgs lowrank_turn_args(const Lowrank &q, bool training);
+template <typename T>
+void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *y, int64_t y_stride, bool training, hipStream_t stream);
+template <typename T>
+void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, int64_t dx_stride, void *da, void *db, hipStream_t stream);
+
+}  // namespace gsdf

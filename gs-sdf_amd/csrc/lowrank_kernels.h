@@ -1,0 +1,803 @@
+// lowrank_kernels.h — the products of the low-rank adapters; lowrank_f32.hip, lowrank_f16.hip and lowrank_bf16.hip compile it for their element type.
+//
+// The adapters' weights are small beside x, base and y, so the operator is bound by the bytes of its rows.  The rows are put in the order of
+// their adapters first (`plan_*`): a tile of 32 rows then has one adapter, and each product is a tile of matrix instructions whose operands
+// come from global memory in the layout that the instruction wants:
+//   shrink   contracts a row's elements (x with A, dy with B^T).  The order of the contraction is free: an instruction's lanes take 64 neighbouring bytes of
+//            each of 16 rows.  The waves of a workgroup split the row and meet in LDS.
+//   expand   contracts ranks (h with B, dh with A^T): the instruction's rows are columns of y, permuted so that a lane holds 16 neighbouring bytes and four lanes 64.
+//   outer    contracts rows (dh with x, h with dy): a lane holds 8 rows x 16 bytes and turns them in registers.
+// h and dh are held in 32 bits.  In front of 16-bit instructions they are split into a high and a low part of the weights' type (16 or 22 bits of the
+// value's), which costs instructions that are not the bound; rounding them once would cost as much precision again as the result's own rounding.
+#pragma once
+#include <type_traits>
+
+#include "lowrank.h"
+
+namespace gsdf {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// ---- pieces of rows ---------------------------------------------------------------------------------------------------------------------------
+// 16 bytes of a row in registers.  Fragments stay whole vectors: as single 16-bit values they would be taken apart, waited for and put together again
+// wherever two paths of the code meet.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(N)));
+};
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::vec load_vec(const T *__restrict__ p) {
+  return *reinterpret_cast<const typename Piece<T, Vec<T>::N>::any *>(p);
+}
+// the elements of a row from k on, 0 behind its end.  There every lane reads its row's first element instead of what is not there: no branch to each
+// element, and the loads leave together.
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::vec load_vec_end(const T *__restrict__ row, int k, int width) {
+  constexpr int N = Vec<T>::N;
+  typename Vec<T>::vec v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = row[k + i < width ? k + i : 0];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = k + i < width ? v[i] : (T)0.f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::vec zero_unless(bool keep, typename Vec<T>::vec v) {
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = keep ? u[i] : 0u;
+  return __builtin_bit_cast(typename Vec<T>::vec, u);
+}
+// N (a multiple of 4) neighbouring results, `valid` of them
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T *__restrict__ p, int valid, const float (&v)[N]) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  if (valid >= N) {
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+      T t[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) t[j] = (T)v[i + j];
+      store_piece<T, W>(p + i, t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < valid) p[i] = (T)v[i];
+  }
+}
+// all ones in the half word (16-bit elements) of each element that stays: sat(bits - (threshold - 1)) is 0 exactly below the threshold
+__device__ __forceinline__ uint32_t keep_mask16(const Dropout &d, uint32_t w) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const unsigned short below = (unsigned short)(d.threshold - 1u);
+  u16x2 t = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w), u16x2{below, below});
+  t = __builtin_elementwise_min(t, u16x2{1, 1});
+  return __builtin_bit_cast(uint32_t, (u16x2)(u16x2{0, 0} - t));
+}
+// zeros where dropped: the 16 bytes of `row` from column `col` on; the survivors' factor goes into the sums
+template <typename V>
+__device__ __forceinline__ V drop8_16(const Dropout &d, uint32_t row, int col, V v) {
+  uint32_t w[4];
+  dropout_bits(d, (uint32_t)col >> 3, row, w);
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] &= keep_mask16(d, w[i]);
+  return __builtin_bit_cast(V, u);
+}
+__device__ __forceinline__ void drop_vec(const Dropout &d, uint32_t row, int col, bf16x8 &v) { v = drop8_16(d, row, col, v); }
+__device__ __forceinline__ void drop_vec(const Dropout &d, uint32_t row, int col, f16x8 &v) { v = drop8_16(d, row, col, v); }
+__device__ __forceinline__ void drop_vec(const Dropout &d, uint32_t row, int col, f32x4 &v) {      // half a block
+  uint32_t w[4];
+  dropout_bits(d, (uint32_t)col >> 3, row, w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = ((i & 1) ? (((col & 4) ? w[2 + i / 2] : w[i / 2]) >> 16) : (((col & 4) ? w[2 + i / 2] : w[i / 2]) & 0xFFFFu)) >= d.threshold ? v[i] : 0.f;
+}
+
+// acc += a b over the 16 bytes of each lane: one 16-bit instruction, or four of 32 bits (any order of the contraction is as good)
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+  return acc;
+}
+// a power of two that brings `largest` into [1, 2): 16-bit numbers of fp16 would run over or vanish
+__device__ __forceinline__ float scale_to_one(float largest) {
+  const int e = (__float_as_int(largest) >> 23) & 255;
+  return e == 0 || e == 255 ? 1.f : __int_as_float((254 - e < 1 ? 1 : 254 - e) << 23);
+}
+
+// ---- shrink: H[place][j] = factor sum_k drop(x)[row][k] W[g][j][k] -------------------------------------------------------------------------
+// A workgroup of `split` waves has a range of rows and its waves take the steps of 128 bytes in turn (one wave: four ranges a workgroup).
+// RT: tiles of 16 ranks.  H: [places][16 RT] (for `expand`) and / or HT: [16 RT][ht_ld] (for `outer`), zeros behind the rank.
+struct ShrinkArgs {
+  const void *x, *w;
+  int64_t x_stride, w_group;      // elements between rows; between the adapters' matrices
+  int width, w_ld, rank, split;
+  const float *scales;            // per adapter, or null
+  float factor;
+  float *h, *ht;
+  int64_t ht_ld;
+  Dropout drop;
+  Plan plan;
+};
+template <typename T, int RT, int TT, bool DROP, bool RAGGED>      // TT: tiles of 16 rows in the range
+__device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, int which, int part, f32x4 *s_sum) {
+  constexpr int RR = RT < 2 ? RT : 2;      // tiles of ranks that meet in LDS at a time
+  typedef typename Vec<T>::vec V;
+  constexpr int N = Vec<T>::N, STEP = 8 * N;
+  const int lane = threadIdx.x & 63, c = lane & 15, quad = lane >> 4;
+  f32x4 acc[RT][TT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T *px[TT];
+  uint32_t row[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {      // a place behind the range reads its last row: its sums are not written
+    const int i = t * 16 + c;
+    row[t] = (uint32_t)q.plan.order[range.y + (i < range.z ? i : range.z - 1)];
+    px[t] = (const T *)q.x + (int64_t)row[t] * q.x_stride;
+  }
+  const T *pw[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int j = r * 16 + c;
+    pw[r] = (const T *)q.w + range.x * q.w_group + (int64_t)(j < q.rank ? j : q.rank - 1) * q.w_ld;
+  }
+  // Ranges begin at different steps: rows of 2^n bytes at the same step would all ask the same memory channels (19 against 15 us for 64 MB).
+  const int full = q.width / STEP, turn = full > 0 ? (int)((unsigned)which % (unsigned)full) : 0;
+  auto column = [&](int step) { return (step + turn < full ? step + turn : step + turn - full) * STEP + quad * N; };
+  auto load = [&](int k, V (&xs)[TT][2], V (&ws)[RT][2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t) xs[t][i] = load_vec<T>(px[t] + k + i * 4 * N);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) ws[r][i] = load_vec<T>(pw[r] + k + i * 4 * N);
+    }
+  };
+  auto add = [&](int k, V (&xs)[TT][2], V (&ws)[RT][2]) {
+    if (DROP) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) drop_vec(q.drop, row[t], k + i * 4 * N, xs[t][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[r][t] = mma(ws[r][i], xs[t][i], acc[r][t]);
+  };
+  constexpr int AHEAD = RT == 1 && TT < 3 ? 4 : RT <= 4 ? 2 : 1;      // steps whose loads are on their way together
+  int s = part;
+  for (; s + (AHEAD - 1) * q.split < full; s += AHEAD * q.split) {
+    V xs[AHEAD][TT][2], ws[AHEAD][RT][2];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load(column(s + u * q.split), xs[u], ws[u]);
+    __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler saves registers and lets two loads go at a time)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) add(column(s + u * q.split), xs[u], ws[u]);
+  }
+  for (; s < full; s += q.split) {
+    V xs[TT][2], ws[RT][2];
+    load(column(s), xs, ws);
+    __builtin_amdgcn_sched_barrier(0);
+    add(column(s), xs, ws);
+  }
+  if (RAGGED && part == full % q.split) {      // the rows' last elements
+    const int k = full * STEP + quad * N;
+    V xs[TT][2], ws[RT][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t) xs[t][i] = load_vec_end<T>(px[t], k + i * 4 * N, q.width);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) ws[r][i] = load_vec_end<T>(pw[r], k + i * 4 * N, q.width);
+    }
+    add(k, xs, ws);
+  }
+  const float f = q.factor * (q.scales != nullptr ? q.scales[range.x] : 1.f);
+  auto put = [&](int r, int t, f32x4 v) {
+    const int i0 = t * 16 + c, j0 = r * 16 + quad * 4;
+    if (i0 >= range.z) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = j0 + i < q.rank ? v[i] * f : 0.f;
+    if (q.h != nullptr) *reinterpret_cast<f32x4 *>(q.h + (int64_t)(range.y + i0) * (16 * RT) + j0) = v;
+    if (q.ht != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.ht[(int64_t)(j0 + i) * q.ht_ld + range.y + i0] = v[i];
+    }
+  };
+  if (q.split == 1) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) put(r, t, acc[r][t]);
+    return;
+  }
+#pragma unroll
+  for (int r0 = 0; r0 < RT; r0 += RR) {      // the waves share the adding and the writing
+    if (r0 > 0) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RR; ++r)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) s_sum[(part * RR * TT + r * TT + t) * 64 + lane] = acc[r0 + r][t];
+    __syncthreads();
+    for (int i = part; i < RR * TT; i += q.split) {
+      f32x4 v = s_sum[i * 64 + lane];
+      for (int w = 1; w < q.split; ++w) v += s_sum[(w * RR * TT + i) * 64 + lane];
+      put(r0 + i / TT, i % TT, v);
+    }
+  }
+}
+template <typename T, int RT, bool DROP, bool RAGGED>      // RAGGED: the width is no multiple of a step
+__global__ void __launch_bounds__(512) lowrank_shrink_kernel(ShrinkArgs q) {
+  extern __shared__ f32x4 s_sum[];      // [split][min(RT, 2)][3][64]
+  const int wave = threadIdx.x >> 6, which = q.split == 1 ? blockIdx.x * 4 + wave : blockIdx.x, part = q.split == 1 ? 0 : wave;
+  if (which >= q.plan.n_ranges) return;
+  const int4 range = q.plan.range[which];
+  if (range.z == 0 || range.x == q.plan.n_adapters) return;
+  if (DROP) dropout_counter(q.drop);
+  if (range.z > 32) shrink_range<T, RT, 3, DROP, RAGGED>(q, range, which, part, s_sum);
+  else if (range.z > 16) shrink_range<T, RT, 2, DROP, RAGGED>(q, range, which, part, s_sum);
+  else shrink_range<T, RT, 1, DROP, RAGGED>(q, range, which, part, s_sum);
+}
+
+// ---- expand: y[row][n] = base[row][n] + sum_j H[place][j] W[g][n][j] -------------------------------------------------------------------------
+// A wave takes 64 columns of a tile at a time: four matrix tiles whose rows are columns of y in the order that
+// leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of them.
+struct ExpandArgs {
+  const float *h;
+  const void *w, *base;
+  void *y;
+  int64_t w_group, base_stride, y_stride;
+  int width, w_ld, rank;
+  bool past;         // y goes past the caches
+  Dropout drop;      // on the result (dx), DROP only
+  Plan plan;
+};
+template <typename T, int RT, int TT, bool DROP, bool RAGGED>
+__device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int turn, int chunks) {
+  typedef typename Vec<T>::vec V;
+  constexpr int N = Vec<T>::N, NB = 16 / N;      // pieces of a lane's 16 columns: piece p at column 4 N p + N quad of the 64
+  constexpr bool WIDE = sizeof(T) == 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
+  const bool idle = range.x == q.plan.n_adapters;
+  if (idle && q.base == q.y) return;      // in place: not touched
+  int64_t row[TT];
+  bool mine[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int i = t * 16 + c;
+    mine[t] = i < range.z;
+    row[t] = q.plan.order[range.y + (mine[t] ? i : range.z - 1)];
+  }
+  const T *base = (const T *)q.base;
+  T *y = (T *)q.y;
+  auto store = [&](T *p, int valid, const float (&v)[N]) {
+    if (!RAGGED || valid >= N) {
+      V o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = (T)v[e];
+      if (q.past) __builtin_nontemporal_store(o, reinterpret_cast<typename Piece<T, N>::any *>(p));
+      else *reinterpret_cast<typename Piece<T, N>::any *>(p) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < valid) p[e] = (T)v[e];
+    }
+  };
+  if (idle) {
+    for (int i = blockIdx.y * 4 + wave; i < chunks; i += gridDim.y * 4) {
+      const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int p = 0; p < NB; ++p) {
+          const int n = ch * 64 + p * 4 * N + quad * N;
+          if ((RAGGED && n >= q.width) || !mine[t]) continue;
+          float v[N];
+          V b;
+          if (base != nullptr) b = !RAGGED || n + N <= q.width ? load_vec<T>(base + row[t] * q.base_stride + n) : load_vec_end<T>(base + row[t] * q.base_stride, n, q.width);
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = base != nullptr ? (float)b[e] : 0.f;
+          store(y + row[t] * q.y_stride + n, q.width - n, v);
+        }
+    }
+    return;
+  }
+  const T *w = (const T *)q.w + range.x * q.w_group;
+  // h of the lane's row as the instruction wants it.  16 bits: 8 ranks a lane, 32 an instruction, high and low parts (a rank of at most 16: both in
+  // one instruction).  32 bits: 4 ranks a lane, 16 a group of four instructions.
+  constexpr int KB = WIDE ? RT : (RT == 1 ? 1 : RT / 2);
+  V hi[TT][KB], lo[TT][KB];
+  float back[TT];
+  auto rank_of = [&](int k) { return WIDE ? k * 16 + quad * 4 : (RT == 1 ? (quad & 1) * 8 : k * 32 + quad * 8); };
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const float *ph = q.h + (int64_t)(range.y + (mine[t] ? t * 16 + c : range.z - 1)) * (16 * RT);
+    f32x4 f[KB][N / 4];
+    float largest = 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        f[k][i] = *reinterpret_cast<const f32x4 *>(ph + rank_of(k) + i * 4);
+        if (DROP) f[k][i] *= q.drop.scale;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(f[k][i][e]));
+      }
+    float down = 1.f;
+    back[t] = 1.f;
+    if (__is_same(T, f16_t)) {
+      largest = fmaxf(largest, __shfl_xor(largest, 16));
+      largest = fmaxf(largest, __shfl_xor(largest, 32));
+      down = scale_to_one(largest);
+      back[t] = 1.f / down;
+    }
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float v = f[k][i / 4][i % 4] * down;
+        const T h = (T)v;
+        const T l = (T)(v - (float)h);
+        hi[t][k][i] = !WIDE && RT == 1 && quad >= 2 ? l : h;
+        lo[t][k][i] = l;
+      }
+  }
+  auto body = [&](int ch, auto columns_whole, auto ranks_whole) {
+    const int n0 = ch * 64 + quad * N;
+    V b[TT][NB], u[4][KB];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int col = ch * 64 + m * 4 / N * 4 * N + (c >> 2) * N + m * 4 % N + (c & 3);      // the column that this lane's weights belong to
+      const T *pw = w + (int64_t)(columns_whole || col < q.width ? col : q.width - 1) * q.w_ld;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const int j = rank_of(k);
+        if (ranks_whole) u[m][k] = load_vec<T>(pw + (j < q.rank ? j : 0));
+        else u[m][k] = load_vec_end<T>(pw, j, q.rank);
+      }
+    }
+    if (base != nullptr) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int p = 0; p < NB; ++p)
+          b[t][p] = columns_whole ? load_vec<T>(base + row[t] * q.base_stride + n0 + p * 4 * N)
+                                  : load_vec_end<T>(base + row[t] * q.base_stride, n0 + p * 4 * N, q.width);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float v[TT][16];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      f32x4 acc[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        if (ranks_whole) u[m][k] = zero_unless<T>(rank_of(k) < q.rank, u[m][k]);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          acc[t] = mma(u[m][k], hi[t][k], acc[t]);
+          if (!WIDE && RT > 1) acc[t] = mma(u[m][k], lo[t][k], acc[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[t][m * 4 + e] = acc[t][e];
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      if (!mine[t]) continue;
+#pragma unroll
+      for (int p = 0; p < NB; ++p) {
+        const int n = n0 + p * 4 * N;
+        float o[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = v[t][p * N + e] * back[t] + (base != nullptr ? (float)b[t][p][e] : 0.f);
+        if (DROP) {
+          uint32_t bits[4];
+          dropout_bits(q.drop, (uint32_t)n >> 3, (uint32_t)row[t], bits);
+          if (N == 4 && (n & 4)) { bits[0] = bits[2]; bits[1] = bits[3]; }
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] = dropout_keeps(q.drop, bits, e) ? o[e] : 0.f;
+        }
+        store(y + row[t] * q.y_stride + n, columns_whole ? N : q.width - n, o);
+      }
+    }
+  };
+  for (int i = blockIdx.y * 4 + wave; i < chunks; i += gridDim.y * 4) {
+    const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
+    if (!RAGGED) body(ch, std::true_type{}, std::true_type{});
+    else if (ch * 64 + 64 <= q.width && q.rank % N == 0) body(ch, std::true_type{}, std::true_type{});
+    else body(ch, std::false_type{}, std::false_type{});
+  }
+}
+template <typename T, int RT, bool DROP, bool RAGGED>      // RAGGED: the width is no multiple of 64 or the rank none of a lane's piece
+__global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT == 4 ? 3 : 2) lowrank_expand_kernel(ExpandArgs q) {
+  const int4 range = q.plan.range[blockIdx.x];
+  if (range.z == 0) return;
+  const int chunks = (q.width + 63) / 64;
+  const int turn = (int)(blockIdx.x % (unsigned)chunks);      // ranges begin at different columns: not all at the same memory channels
+  if (DROP) dropout_counter(q.drop);
+  if (range.z > 32) expand_range<T, RT, 3, DROP, RAGGED>(q, range, turn, chunks);
+  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED>(q, range, turn, chunks);
+  else expand_range<T, RT, 1, DROP, RAGGED>(q, range, turn, chunks);
+}
+
+// ---- outer: sum over an adapter's rows of UT[j][place] V[row][c] ----------------------------------------------------------------------------
+// A workgroup of 8 waves owns a chunk of rows and 16 lanes x 16 bytes of columns; its waves take 32 rows in turn and meet in LDS.
+struct OuterSide {
+  const float *ut;      // [..][ut_ld]
+  const void *v;
+  int64_t v_stride;
+  int width, drop;
+  int columns_first;    // result [g][c][j] (B) instead of [g][j][c] (A)
+  void *out;
+  float *part;          // [slots][16 RT ranks][width] or [slots][width][16 RT]
+};
+struct OuterArgs {
+  OuterSide side[2];
+  int64_t ut_ld;
+  int rank, rank_padded, blocks0, blocks;      // column blocks of side 0, of both
+  Dropout drop;
+  Plan plan;
+};
+// element e of 8 rows as one fragment
+__device__ __forceinline__ u32x4 column_of(const u32x4 (&v)[8], int e) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+  return o;
+}
+template <typename T, int RT, bool RAGGED>      // RAGGED: a width is no multiple of COLS
+__global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
+  typedef typename Vec<T>::vec V;
+  constexpr int VE = Vec<T>::N, COLS = 16 * VE;      // elements of a lane's piece, columns of a workgroup
+  __shared__ f32x4 s_sum[4][VE][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
+  const int block = blockIdx.x % q.blocks;
+  const int4 chunk = q.plan.chunk[blockIdx.x / q.blocks];
+  if (chunk.z == 0) return;
+  const bool second = block >= q.blocks0;
+  const OuterSide &s = q.side[second];
+  const int col0 = (block - (second ? q.blocks0 : 0)) * COLS, col = col0 + c * VE, valid = s.width - col;
+  const int rank0 = blockIdx.y * 64;
+  const bool drop = s.drop != 0;
+  if (drop) dropout_counter(q.drop);
+  f32x4 acc[RT][VE];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (chunk.z + 31) / 32;
+  const int *order = q.plan.order + chunk.y;
+  const bool columns_whole = !RAGGED || col0 + COLS <= s.width;
+  for (int st = wave; st < steps; st += 8) {
+    const int at = st * 32 + quad * 8;       // the lane's 8 rows
+    int row[8];
+    V v[8];
+    f32x4 u[RT][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = order[at + i < chunk.z ? at + i : chunk.z - 1];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {      // (places behind the chunk are in the buffer, which has room behind its last)
+      const float *pu = s.ut + (int64_t)(rank0 + r * 16 + c) * q.ut_ld + chunk.y;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) u[r][i] = load_vec<float>(pu + at + i * 4);
+    }
+    if (columns_whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = load_vec<T>((const T *)s.v + (int64_t)row[i] * s.v_stride + col);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = load_vec_end<T>((const T *)s.v + (int64_t)row[i] * s.v_stride, col, s.width);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (drop) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) drop_vec(q.drop, (uint32_t)row[i], col, v[i]);
+    }
+    if (st * 32 + 32 > chunk.z) {      // rows behind the chunk: nothing, whatever was read in their place
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = zero_unless<T>(at + i < chunk.z, v[i]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) u[r][i / 4][i % 4] = at + i < chunk.z ? u[r][i / 4][i % 4] : 0.f;
+      }
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[r][i / 4][i % 4], v[i][e], acc[r][e], 0, 0, 0);
+    } else {
+      constexpr bool HALF = __is_same(T, f16_t);
+      float down = 1.f, up = 1.f;
+      if (HALF) {      // one power of two for the step: the sums of other steps keep their own
+        float largest = 0.f;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(u[r][i / 4][i % 4]));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o));
+        down = scale_to_one(largest);
+        up = 1.f / down;
+      }
+      V hi[RT], lo[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float t = u[r][i / 4][i % 4] * down;
+          hi[r][i] = (T)t;
+          lo[r][i] = (T)(t - (float)hi[r][i]);
+        }
+      u32x4 words[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) words[i] = __builtin_bit_cast(u32x4, v[i]);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const V b = __builtin_bit_cast(V, column_of(words, e));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if (HALF) {
+            f32x4 t = mma(lo[r], b, f32x4{0.f, 0.f, 0.f, 0.f});
+            t = mma(hi[r], b, t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[r][e][i] = fmaf(t[i], up, acc[r][e][i]);
+          } else {
+            acc[r][e] = mma(lo[r], b, acc[r][e]);
+            acc[r][e] = mma(hi[r], b, acc[r][e]);
+          }
+        }
+      }
+    }
+  }
+  // the waves' sums: 4 + 4, 2 + 2, 1 + 1, one tile of ranks at a time
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    for (int half = 4; half > 0; half >>= 1) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s_sum[wave - half][e][lane] = acc[r][e];
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[r][e] += s_sum[wave][e][lane];
+      }
+    }
+  }
+  if (wave != 0 || valid <= 0) return;
+  const float f = drop ? q.drop.scale : 1.f;
+  const int RP = q.rank_padded;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int j0 = rank0 + r * 16 + quad * 4;
+    if (j0 >= q.rank) continue;
+    if (!s.columns_first) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (j0 + i >= q.rank) continue;
+        float o[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o[e] = acc[r][e][i] * f;
+        if (chunk.w < 0) store_some<T, VE>((T *)s.out + ((int64_t)chunk.x * q.rank + j0 + i) * s.width + col, valid, o);
+        else store_some<float, VE>(s.part + ((int64_t)chunk.w * RP + j0 + i) * s.width + col, valid, o);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        if (e >= valid) continue;
+        const float o[4] = {acc[r][e][0] * f, acc[r][e][1] * f, acc[r][e][2] * f, acc[r][e][3] * f};
+        if (chunk.w < 0) store_some<T, 4>((T *)s.out + ((int64_t)chunk.x * s.width + col + e) * q.rank + j0, q.rank - j0, o);
+        else store_some<float, 4>(s.part + ((int64_t)chunk.w * s.width + col + e) * RP + j0, 4, o);
+      }
+    }
+  }
+}
+// the adapters that `outer` did not finish: the sum of several chunks, in their order, or zeros where there are no rows
+struct SumArgs {
+  OuterSide side[2];
+  int rank, rank_padded, blocks0;
+  Plan plan;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) lowrank_sum_kernel(SumArgs q) {
+  const bool second = (int)blockIdx.x >= q.blocks0;
+  const OuterSide &s = q.side[second];
+  const int g = blockIdx.y;
+  const int2 slots = q.plan.slots[g];
+  if (slots.y == 1) return;
+  const int64_t i = (int64_t)((int)blockIdx.x - (second ? q.blocks0 : 0)) * 256 + threadIdx.x, n = (int64_t)q.rank * s.width;
+  if (i >= n) return;
+  float v = 0.f;
+  if (slots.y > 1) {
+    const int64_t each = (int64_t)q.rank_padded * s.width;
+    const int64_t at = s.columns_first ? i / q.rank * q.rank_padded + i % q.rank : i;
+    const float *p = s.part + slots.x * each + at;
+    int k = 0;
+    for (; k + 8 <= slots.y; k += 8) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = p[(k + i) * each];
+      v += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+    }
+    for (; k < slots.y; ++k) v += p[k * each];
+  }
+  ((T *)s.out)[g * n + i] = (T)v;
+}
+
+// ---- a few rows without gradients: no order, a workgroup per row ----------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(1024) lowrank_row_shrink_kernel(Ids ids, const T *__restrict__ x, int64_t x_stride, const T *__restrict__ a, int width, int rank,
+                                                                  const float *__restrict__ scales, Dropout drop, float *__restrict__ h) {
+  typedef typename Vec<T>::vec V;
+  constexpr int N = Vec<T>::N;
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, j = blockIdx.y * 16 + (threadIdx.x >> 6), g = group_of(ids, row);
+  if (j >= rank || g == ids.n_adapters) return;
+  dropout_counter(drop);
+  const T *px = x + row * x_stride, *pa = a + ((int64_t)g * rank + j) * width;
+  float s = 0.f;
+  auto add = [&](int k, V u, V v) {
+    if (drop.threshold != 0) drop_vec(drop, (uint32_t)row, k, u);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s = fmaf((float)u[i], (float)v[i], s);
+  };
+  int k = lane * N;
+  for (; k + 192 * N + N <= width; k += 256 * N) {      // four pieces on their way together
+    V u[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { u[i] = load_vec<T>(px + k + i * 64 * N); v[i] = load_vec<T>(pa + k + i * 64 * N); }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(k + i * 64 * N, u[i], v[i]);
+  }
+  for (; k + N <= width; k += 64 * N) add(k, load_vec<T>(px + k), load_vec<T>(pa + k));
+  if (k < width) add(k, load_vec_end<T>(px, k, width), load_vec_end<T>(pa, k, width));
+  s = wave_sum_to_lane63(s);
+  if (lane == 63) h[row * rank + j] = s * (scales != nullptr ? scales[g] : 1.f) * (drop.threshold != 0 ? drop.scale : 1.f);
+}
+// 64 columns a step, four lanes to a column
+template <typename T>
+__global__ void __launch_bounds__(256) lowrank_row_expand_kernel(Ids ids, const float *__restrict__ h, const T *__restrict__ b, int width, int rank, const T *base,
+                                                                 int64_t base_stride, T *y, int64_t y_stride) {
+  constexpr int N = Vec<T>::N;
+  const int64_t row = blockIdx.x;
+  const int g = group_of(ids, row), sub = threadIdx.x & 3;
+  if (g == ids.n_adapters && base == y) return;
+  const float *ph = h + row * rank;
+  for (int n = blockIdx.y * 64 + (threadIdx.x >> 2); n < width; n += gridDim.y * 64) {
+    const float add = base != nullptr ? (float)base[row * base_stride + n] : 0.f;
+    float s = 0.f;
+    if (g < ids.n_adapters) {
+      const T *pb = b + ((int64_t)g * width + n) * rank;
+      for (int j = sub * N; j < rank; j += 4 * N) {
+        const typename Vec<T>::vec v = j + N <= rank ? load_vec<T>(pb + j) : load_vec_end<T>(pb, j, rank);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s = fmaf(j + i < rank ? ph[j + i] : 0.f, (float)v[i], s);
+      }
+    }
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    if (sub == 0) y[row * y_stride + n] = (T)(s + add);
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------------------------
+static constexpr int64_t LR_FEW_ROWS = 64;
+static constexpr int64_t LR_PAST = 32 << 20;      // bytes of a result from which on it is written past the caches
+
+#define GSDF_BY_RANK(rt, ...)                                 \
+  switch (rt) {                                               \
+    case 1: { constexpr int RT = 1; __VA_ARGS__; break; }     \
+    case 2: { constexpr int RT = 2; __VA_ARGS__; break; }     \
+    case 4: { constexpr int RT = 4; __VA_ARGS__; break; }     \
+    default: { constexpr int RT = 8; __VA_ARGS__; break; }    \
+  }
+
+template <typename T>
+static void shrink_launch(const Lowrank &q, const void *x, int64_t x_stride, int width, const void *w, int64_t w_group, int w_ld, const float *scales, bool drop, float *h,
+                          float *ht, hipStream_t stream) {
+  ShrinkArgs s;
+  s.x = x; s.w = w; s.x_stride = x_stride; s.w_group = w_group; s.width = width; s.w_ld = w_ld; s.rank = q.a.rank;
+  s.scales = scales; s.factor = drop ? q.drop.scale : 1.f; s.h = h; s.ht = ht; s.ht_ld = q.ht_ld; s.drop = q.drop; s.plan = q.plan;
+  const int steps = (int)ceil_div(width, 128 / (int)sizeof(T));
+  s.split = steps >= 8 ? 8 : steps >= 4 ? 4 : steps >= 2 ? 2 : 1;
+  const unsigned grid = (unsigned)(s.split == 1 ? ceil_div(q.plan.n_ranges, 4) : q.plan.n_ranges), threads = s.split == 1 ? 256 : 64 * s.split;
+  const bool ragged = width % (128 / (int)sizeof(T)) != 0;
+  GSDF_BY_RANK(q.rt, {
+    const size_t lds = s.split == 1 ? 0 : (size_t)s.split * (RT < 2 ? 1 : 2) * 3 * 64 * sizeof(f32x4);
+    if (drop && ragged) lowrank_shrink_kernel<T, RT, true, true><<<grid, threads, lds, stream>>>(s);
+    else if (drop) lowrank_shrink_kernel<T, RT, true, false><<<grid, threads, lds, stream>>>(s);
+    else if (ragged) lowrank_shrink_kernel<T, RT, false, true><<<grid, threads, lds, stream>>>(s);
+    else lowrank_shrink_kernel<T, RT, false, false><<<grid, threads, lds, stream>>>(s);
+  });
+}
+template <typename T>
+static void expand_launch(const Lowrank &q, const float *h, const void *w, int64_t w_group, int w_ld, int ranks, int width, const void *base,
+                          int64_t base_stride, void *y, int64_t y_stride, bool drop, hipStream_t stream) {
+  ExpandArgs s;
+  s.h = h; s.w = w; s.base = base; s.y = y; s.w_group = w_group; s.base_stride = base_stride; s.y_stride = y_stride; s.width = width; s.w_ld = w_ld; s.rank = ranks;
+  s.drop = q.drop; s.plan = q.plan;
+  s.past = (int64_t)q.a.rows * width * (int64_t)sizeof(T) >= LR_PAST;
+  const int64_t chunks = ceil_div(width, 64);
+  const dim3 grid((unsigned)q.plan.n_ranges, (unsigned)ceil_div(chunks, chunks >= 16 ? 16 : 4));
+  const bool ragged = width % 64 != 0 || ranks % (16 / (int)sizeof(T)) != 0;
+  GSDF_BY_RANK(q.rt, {
+    if (drop && ragged) lowrank_expand_kernel<T, RT, true, true><<<grid, 256, 0, stream>>>(s);
+    else if (drop) lowrank_expand_kernel<T, RT, true, false><<<grid, 256, 0, stream>>>(s);
+    else if (ragged) lowrank_expand_kernel<T, RT, false, true><<<grid, 256, 0, stream>>>(s);
+    else lowrank_expand_kernel<T, RT, false, false><<<grid, 256, 0, stream>>>(s);
+  });
+}
+
+template <typename T>
+void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *y, int64_t y_stride, bool training, hipStream_t stream) {
+  const gsdf_lowrank_args &a = q.a;
+  const Ids ids = {a.ids, a.ids_64, a.n_adapters};
+  if (!training && a.rows <= LR_FEW_ROWS) {
+    lowrank_row_shrink_kernel<T><<<dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, 16)), 1024, 0, stream>>>(ids, (const T *)a.x, a.x_stride, (const T *)a.a, a.n_in, a.rank,
+                                                                                                         a.scales, q.drop, q.h);
+    lowrank_row_expand_kernel<T><<<dim3((unsigned)a.rows, (unsigned)(ceil_div(a.n_out, 64) < 4096 ? ceil_div(a.n_out, 64) : 4096)), 256, 0, stream>>>(
+        ids, q.h, (const T *)a.b, a.n_out, a.rank, (const T *)base,
+                                                                                                         base_stride, (T *)y, y_stride);
+    return;
+  }
+  lowrank_plan_launch(q.plan, ids, lowrank_turn_args(q, training), stream);
+  shrink_launch<T>(q, a.x, a.x_stride, a.n_in, a.a, (int64_t)a.rank * a.n_in, a.n_in, a.scales, q.drop.threshold != 0, q.h, training ? q.ht : nullptr, stream);
+  expand_launch<T>(q, q.h, a.b, (int64_t)a.n_out * a.rank, a.rank, a.rank, a.n_out, base, base_stride, y, y_stride, false, stream);
+}
+
+template <typename T>
+void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, int64_t dx_stride, void *da, void *db, hipStream_t stream) {
+  const gsdf_lowrank_args &a = q.a;
+  const bool drop = q.drop.threshold != 0;
+  const unsigned G = (unsigned)a.n_adapters;
+  if (a.rows > 0 && (dx != nullptr || da != nullptr))
+    shrink_launch<T>(q, dy, dy_stride, a.n_out, q.turned[1], (int64_t)a.rank * a.n_out, a.n_out, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr, stream);
+  if (a.rows > 0 && dx != nullptr)
+    expand_launch<T>(q, q.dh, q.turned[0], (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride, drop, stream);
+  if (da == nullptr && db == nullptr) return;
+  constexpr int COLS = 16 * (16 / (int)sizeof(T));
+  OuterArgs o;
+  o.side[0] = {q.dht, a.x, a.x_stride, a.n_in, drop, 0, da, q.part[0]};
+  o.side[1] = {q.ht, dy, dy_stride, a.n_out, 0, 1, db, q.part[1]};
+  o.ut_ld = q.ht_ld; o.rank = a.rank; o.rank_padded = q.rp; o.drop = q.drop; o.plan = q.plan;
+  o.blocks0 = da != nullptr ? (int)ceil_div(a.n_in, COLS) : 0;
+  const unsigned blocks1 = db != nullptr ? (unsigned)ceil_div(a.n_out, COLS) : 0;
+  o.blocks = o.blocks0 + (int)blocks1;
+  if (a.rows > 0) {
+    const dim3 grid((unsigned)o.blocks * (unsigned)q.plan.max_chunks, q.rt == 8 ? 2 : 1);
+    const bool ragged = a.n_in % COLS != 0 || a.n_out % COLS != 0;
+    switch (q.rt) {
+      case 1: ragged ? lowrank_outer_kernel<T, 1, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 1, false><<<grid, 512, 0, stream>>>(o); break;
+      case 2: ragged ? lowrank_outer_kernel<T, 2, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 2, false><<<grid, 512, 0, stream>>>(o); break;
+      default: ragged ? lowrank_outer_kernel<T, 4, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 4, false><<<grid, 512, 0, stream>>>(o); break;
+    }
+  }
+  SumArgs s;
+  s.side[0] = o.side[0]; s.side[1] = o.side[1]; s.rank = a.rank; s.rank_padded = q.rp; s.plan = q.plan;
+  s.blocks0 = da != nullptr ? (int)ceil_div((int64_t)a.rank * a.n_in, 256) : 0;
+  const unsigned sum1 = db != nullptr ? (unsigned)ceil_div((int64_t)a.rank * a.n_out, 256) : 0;
+  lowrank_sum_kernel<T><<<dim3((unsigned)s.blocks0 + sum1, G), 256, 0, stream>>>(s);
+}
+
+
+}  // namespace gsdf
