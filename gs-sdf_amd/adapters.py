@@ -27,15 +27,20 @@ def _need(cond, what):
 
 
 def _same(ref, t, name, dtype=None):
-    _need(isinstance(t, torch.Tensor), f"{name}: expected a tensor")
-    _need(t.device == ref.device, f"{name}: expected a tensor on {ref.device}, got one on {t.device}")
-    _need(dtype is None or t.dtype == dtype, f"{name}: expected dtype {dtype}, got {t.dtype}")
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name}: expected a tensor")
+    if t.device != ref.device:
+        raise RuntimeError(f"{name}: expected a tensor on {ref.device}, got one on {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
 
 
 def _elements(t, name):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: expected a device tensor (the HIP path has no CPU fallback)")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise RuntimeError(f"{name}: expected a device tensor (the HIP path has no CPU fallback)")
     d = _DTYPES.get(t.dtype)
-    _need(d is not None, f"{name}: expected fp32, fp16 or bf16 elements, got {t.dtype}")
+    if d is None:
+        raise RuntimeError(f"{name}: expected fp32, fp16 or bf16 elements, got {t.dtype}")
     return d
 
 
@@ -50,7 +55,8 @@ def _rows(t):
 
 def _index(t, ref, name):
     _same(ref, t, name)
-    _need(t.dtype in (torch.int32, torch.int64), f"{name}: expected int32 or int64, got {t.dtype}")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name}: expected int32 or int64, got {t.dtype}")
     return t.contiguous()
 
 
@@ -60,13 +66,16 @@ def _offset(offset, ref):
         _same(ref, offset, "offset", torch.int64)
         _need(offset.numel() == 1, "offset: expected one device word")
         return 0, offset
-    _need(0 <= int(offset) < 2 ** 64, "offset: expected a number in [0, 2^64)")
+    if not 0 <= int(offset) < 2 ** 64:
+        raise RuntimeError("offset: expected a number in [0, 2^64)")
     return int(offset), None
 
 
 def _check_p(p, seed):
-    _need(0.0 <= float(p) <= 1.0, f"p: expected a probability in [0, 1], got {p}")
-    _need(0 <= int(seed) < 2 ** 64, "seed: expected a number in [0, 2^64)")
+    if not 0.0 <= float(p) <= 1.0:
+        raise RuntimeError(f"p: expected a probability in [0, 1], got {p}")
+    if not 0 <= int(seed) < 2 ** 64:
+        raise RuntimeError("seed: expected a number in [0, 2^64)")
 
 
 def _run(dev, fn, *args):
@@ -85,7 +94,20 @@ def _ptr(t):
 
 
 def _grad_wanted(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _once(backward):
+    """a backward pass that is not differentiated again (torch.autograd.function.once_differentiable, whose cost only a call with create_graph pays)"""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 # ------------------------------------------------------------------------------------------------
@@ -118,7 +140,7 @@ class _Lowrank(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, a, b, ids, scales, save, word = ctx.saved_tensors
         dtype, p, seed, offset = ctx.rest
@@ -141,23 +163,28 @@ def _lowrank_checked(x, a, b, ids, scales, base, p, seed, offset):
     dtype = _elements(x, "x")
     _same(x, a, "a", x.dtype)
     _same(x, b, "b", x.dtype)
-    _need(x.dim() >= 1 and a.dim() == 3 and b.dim() == 3, "lowrank_adapt: expected x [..., k], a [g, r, k], b [g, n, r]")
-    (g, r, k), n = a.shape, b.shape[1]
-    _need(x.shape[-1] == k and b.shape[0] == g and b.shape[2] == r,
-          f"lowrank_adapt: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not fit (x [..., k], a [g, r, k], b [g, n, r])")
-    _need(1 <= r <= MAX_RANK, f"lowrank_adapt: rank {r} outside [1, {MAX_RANK}]")
-    _need(1 <= g <= MAX_ADAPTERS, f"lowrank_adapt: {g} adapters outside [1, {MAX_ADAPTERS}]")
-    _need(k >= 1 and n >= 1, "lowrank_adapt: an empty projection")
+    if x.dim() < 1 or a.dim() != 3 or b.dim() != 3:
+        raise RuntimeError("lowrank_adapt: expected x [..., k], a [g, r, k], b [g, n, r]")
+    (g, r, k), lead = a.shape, x.shape[:-1]
+    n = b.shape[1]
+    if x.shape[-1] != k or b.shape[0] != g or b.shape[2] != r:
+        raise RuntimeError(f"lowrank_adapt: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not fit (x [..., k], a [g, r, k], b [g, n, r])")
+    if not (1 <= r <= MAX_RANK and 1 <= g <= MAX_ADAPTERS and k >= 1 and n >= 1):
+        raise RuntimeError(f"lowrank_adapt: rank {r} outside [1, {MAX_RANK}], {g} adapters outside [1, {MAX_ADAPTERS}], or an empty projection {k} -> {n}")
     ids = _index(ids, x, "ids")
-    _need(ids.shape == x.shape[:-1], f"ids: expected shape {tuple(x.shape[:-1])}, got {tuple(ids.shape)}")
+    if ids.shape != lead:
+        raise RuntimeError(f"ids: expected shape {tuple(lead)}, got {tuple(ids.shape)}")
     if scales is not None:
         _same(x, scales, "scales", torch.float32)
-        _need(tuple(scales.shape) == (g,), f"scales: expected shape ({g},), got {tuple(scales.shape)}")
-        _need(not (torch.is_grad_enabled() and scales.requires_grad), "scales: constants, no gradient is offered for them")
+        if scales.dim() != 1 or scales.shape[0] != g:
+            raise RuntimeError(f"scales: expected shape ({g},), got {tuple(scales.shape)}")
+        if scales.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("scales: constants, no gradient is offered for them")
         scales = scales.contiguous()
     if base is not None:
         _same(x, base, "base", x.dtype)
-        _need(base.shape == x.shape[:-1] + (n,), f"base: expected shape {tuple(x.shape[:-1]) + (n,)}, got {tuple(base.shape)}")
+        if base.dim() != x.dim() or base.shape[-1] != n or base.shape[:-1] != lead:
+            raise RuntimeError(f"base: expected shape {tuple(lead) + (n,)}, got {tuple(base.shape)}")
     _check_p(p, seed)
     return dtype, a.contiguous(), b.contiguous(), ids, scales, _offset(offset, x)
 
@@ -239,7 +266,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, residual, dtype, p, seed, offset, word)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         word, = ctx.saved_tensors
         dtype, p, seed, offset = ctx.rest
@@ -289,7 +316,7 @@ class _Balance(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, v_loss, _v_counts):
         m, mask, pull = ctx.saved_tensors
         rows, e = m.shape

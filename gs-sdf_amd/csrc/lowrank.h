@@ -7,6 +7,7 @@ namespace gsdf {
 static constexpr int LR_CUS = 256;          // compute units the ranges are dealt to
 static constexpr int LR_AIM = 40;           // rows of a range that are aimed at, at most
 static constexpr int LR_RANGE = 48;         // most rows of a range: three matrix tiles
+static constexpr int LR_WIDE = 64;           // most rows of a range of `expand`
 static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
 
 // ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------
@@ -14,11 +15,12 @@ static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
 struct Plan {
   int *order;      // [rows]: the row at each place, adapters one behind the other, rows of one adapter in their own order
   int4 *range;     // [n_ranges]: adapter, first place, rows (0: unused), -
+  int4 *wide;      // [n_wide]: the same of up to LR_WIDE rows
   int4 *chunk;     // [max_chunks]: adapter, first place, rows (0: unused), slot of its partial sums (-1: the adapter's only chunk)
   int2 *slots;     // [n_adapters]: first slot, chunks
   int *hist;       // [blocks][n_adapters]: rows of each adapter in each workgroup's share
   int rows, n_adapters, blocks, block_rows;
-  int per, wanted, n_ranges, max_chunks;
+  int per, wanted, n_ranges, n_wide, max_chunks;
 };
 // Every range costs a compute unit about the bytes of its rows and of its adapter's weights, and ends with its adapter: `per` is the smallest size from
 // this one on that makes no more ranges than a multiple of the units (264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 take 20: 8192 rows of 8 KB).
@@ -33,10 +35,12 @@ static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int 
   if (p->per < least) p->per = least;
   const int64_t most = rows / LR_RANGE + n_adapters + 1;
   p->n_ranges = (int)(p->wanted > most ? p->wanted : most);
+  p->n_wide = (int)(rows / LR_WIDE + n_adapters + 1);
   p->max_chunks = (int)(rows / LR_CHUNK + n_adapters);
   char *at = (char *)mem;
   auto take = [&](size_t bytes) { char *r = at; at += align_up(bytes, 16); return r; };
   p->range = (int4 *)take((size_t)p->n_ranges * 16);
+  p->wide = (int4 *)take((size_t)p->n_wide * 16);
   p->chunk = (int4 *)take((size_t)p->max_chunks * 16);
   p->slots = (int2 *)take((size_t)n_adapters * 8);
   p->hist = (int *)take((size_t)p->blocks * n_adapters * 4);
@@ -58,15 +62,18 @@ __device__ __forceinline__ int group_of(Ids ids, int64_t row) {
   return g >= 0 && g < ids.n_adapters ? (int)g : ids.n_adapters;
 }
 
-// ---- weights turned for the backward pass: A [g][r][k] -> [g][k][RP] (zeros behind the rank), B [g][n][r] -> [g][r][n] ----------------------
-// They go with the launch that begins the plan, which leaves the rest of the card idle.
-struct TurnArgs {
-  const void *in[2];
-  void *out[2];
-  int rows[2], cols[2], out_ld[2];      // of one adapter's matrix, and of the turned one
-  int blocks0, blocks;                  // tiles of 64 x 64 of the first matrix, of both
-  int es;
+// ---- weights laid out for the matrix instructions ----------------------------------------------------------------------------------------
+// `shrink` reads fragments: [adapter][step][tile of 16 ranks][2][64 lanes] pieces of 16 bytes, lane (c, quad) of half i with the elements
+// step 8N + i 4N + quad N .. of rank c of the tile (N elements in 16 bytes; zeros behind the width and the rank).  A wave's load is 1 KB of neighbours, where 16 rows
+// 2^n bytes apart ask one channel of the L2 (rank 64, 8192 rows of 8 KB: 26 us against 22; rank 128: 41 against 28).  `expand` of the backward pass
+// reads A^T as [adapter][n_in][RP].  They are made beside the plan, whose few workgroups leave the card idle.
+struct PackArgs {
+  const void *a, *b;
+  void *a_frag, *b_frag, *a_turned;      // a_turned, b_frag: null without a backward pass
+  int n_in, n_out, rank, rt, es;
+  int blocks[3], n_blocks;               // workgroups of each for one adapter; of all for all
 };
+
 // a call, with everything in its place
 struct Lowrank {
   gsdf_lowrank_args a;
@@ -76,14 +83,15 @@ struct Lowrank {
   int64_t ht_ld;
   // saved by the forward pass (beside the plan)
   float *ht;
-  void *turned[2];
+  void *b_frag, *a_turned;
   // workspace
   float *h, *dh, *dht, *part[2];
+  void *a_frag;
   size_t save_bytes, fwd_ws_bytes, bwd_ws_bytes;
 };
 
-void lowrank_plan_launch(const Plan &p, const Ids &ids, const TurnArgs &turn, hipStream_t stream);
-TurnArgs lowrank_turn_args(const Lowrank &q, bool training);
+void lowrank_plan_launch(const Plan &p, const Ids &ids, const PackArgs &pack, hipStream_t stream);
+PackArgs lowrank_pack_args(const Lowrank &q, bool training);
 template <typename T>
 void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *y, int64_t y_stride, bool training, hipStream_t stream);
 template <typename T>

@@ -6,26 +6,35 @@
 
 namespace gsdf {
 
-// exclusive sums of (a, b, c) over the 1024 threads of the workgroup; totals in `sum`
-__device__ __forceinline__ int3 block_scan3(int3 v, int3 *sum, int (*s_w)[3]) {
+// exclusive sums of C numbers over the 1024 threads of the workgroup; totals in `sum`
+template <int C>
+__device__ __forceinline__ void block_scan(int (&v)[C], int (&sum)[C], int (*s_w)[4]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int3 i = v;
+  int i[C], before[C];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int a = __shfl_up(i.x, o), b = __shfl_up(i.y, o), c = __shfl_up(i.z, o);
-    if (lane >= o) { i.x += a; i.y += b; i.z += c; }
-  }
-  if (lane == 63) { s_w[wave][0] = i.x; s_w[wave][1] = i.y; s_w[wave][2] = i.z; }
-  __syncthreads();
-  int3 before = {0, 0, 0}, all = {0, 0, 0};
+  for (int c = 0; c < C; ++c) { i[c] = v[c]; before[c] = sum[c] = 0; }
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    if (w == wave) before = all;
-    all.x += s_w[w][0]; all.y += s_w[w][1]; all.z += s_w[w][2];
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int u = __shfl_up(i[c], o);
+      i[c] += lane >= o ? u : 0;
+    }
+  if (lane == 63) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) s_w[wave][c] = i[c];
   }
   __syncthreads();
-  *sum = all;
-  return {before.x + i.x - v.x, before.y + i.y - v.y, before.z + i.z - v.z};
+#pragma unroll
+  for (int w = 0; w < 16; ++w)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      before[c] = w == wave ? sum[c] : before[c];
+      sum[c] += s_w[w][c];
+    }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < C; ++c) v[c] = before[c] + i[c] - v[c];
 }
 // the last group that begins at or before i
 __device__ __forceinline__ int find_group(const int *first, int n, int i) {
@@ -38,33 +47,52 @@ __device__ __forceinline__ int find_group(const int *first, int n, int i) {
 }
 
 template <typename E>
-__device__ __forceinline__ void turn_tile(const TurnArgs &q, int block, E *s) {      // 1024 threads; s: [64][65]
-  const int g = block / q.blocks, in_g = block % q.blocks, k = in_g >= q.blocks0;
-  const int tiles_c = (q.cols[k] + 63) / 64, b = in_g - (k ? q.blocks0 : 0), r0 = b / tiles_c * 64, c0 = b % tiles_c * 64;
-  const E *in = (const E *)q.in[k] + (int64_t)g * q.rows[k] * q.cols[k];
-  E *out = (E *)q.out[k] + (int64_t)g * q.cols[k] * q.out_ld[k];
+__device__ __forceinline__ void pack_block(const PackArgs &q, int block) {
+  typedef E vec __attribute__((ext_vector_type(16 / sizeof(E))));
+  constexpr int N = 16 / sizeof(E);
+  const int each = q.blocks[0] + q.blocks[1] + q.blocks[2], g = block / each;
+  int b = block % each;
+  const E *a = (const E *)q.a + (int64_t)g * q.rank * q.n_in, *bm = (const E *)q.b + (int64_t)g * q.n_out * q.rank;
+  vec v;
+  if (b < q.blocks[0] + q.blocks[1]) {      // fragments of A, or of B^T
+    const bool second = b >= q.blocks[0];
+    const int p = (b - (second ? q.blocks[0] : 0)) * 1024 + threadIdx.x, width = second ? q.n_out : q.n_in, steps = (width + 8 * N - 1) / (8 * N);
+    const int lane = p & 63, r = (p >> 7) & (q.rt - 1), step = (p >> 7) / q.rt;
+    if (step >= steps) return;
+    const int j = r * 16 + (lane & 15), k = step * 8 * N + ((p >> 6) & 1) * 4 * N + (lane >> 4) * N;
+    if (!second && j < q.rank && k + N <= width) v = *reinterpret_cast<const typename Piece<E, N>::any *>(a + (int64_t)j * width + k);
+    else
 #pragma unroll
-  for (int i = threadIdx.x; i < 4096; i += 1024) {
-    const int r = r0 + i / 64, c = c0 + i % 64;
-    s[i / 64 * 65 + i % 64] = r < q.rows[k] && c < q.cols[k] ? in[(int64_t)r * q.cols[k] + c] : (E)0;
-  }
-  __syncthreads();
+    for (int i = 0; i < N; ++i) {
+      const bool in = j < q.rank && k + i < width;
+      const int64_t at = in ? (second ? (int64_t)(k + i) * q.rank + j : (int64_t)j * width + k + i) : 0;
+      const E t = second ? bm[at] : a[at];
+      v[i] = in ? t : (E)0;
+    }
+    reinterpret_cast<vec *>(second ? q.b_frag : q.a_frag)[((int64_t)g * steps * q.rt << 7) + p] = v;
+  } else {                                   // A^T: neighbouring lanes have neighbouring columns of A
+    b -= q.blocks[0] + q.blocks[1];
+    const int p = b * 1024 + threadIdx.x, jp = p / q.n_in, k = p % q.n_in, per_row = q.rt * 16 / N;
+    if (jp >= per_row) return;
 #pragma unroll
-  for (int i = threadIdx.x; i < 4096; i += 1024) {
-    const int c = c0 + i / 64, r = r0 + i % 64;
-    if (c < q.cols[k] && r < q.out_ld[k]) out[(int64_t)c * q.out_ld[k] + r] = s[i % 64 * 65 + i / 64];
+    for (int i = 0; i < N; ++i) {
+      const int j = jp * N + i;
+      const E t = a[j < q.rank ? (int64_t)j * q.n_in + k : 0];
+      v[i] = j < q.rank ? t : (E)0;
+    }
+    reinterpret_cast<vec *>(q.a_turned)[((int64_t)g * q.n_in + k) * per_row + jp] = v;
   }
-}
-__device__ __forceinline__ void turn_block(const TurnArgs &q, int block, int *s) {
-  if (q.es == 4) turn_tile<uint32_t>(q, block, (uint32_t *)s);
-  else turn_tile<unsigned short>(q, block, (unsigned short *)s);
 }
 
 // The plan takes two launches: each workgroup counts its share of the rows; then each adds up the counts of all (they are few), finds where its own rows
 // go and puts them there.  One workgroup alone took 13 us for 8192 rows.
-__global__ void __launch_bounds__(1024) lowrank_plan_count_kernel(Plan p, Ids ids, TurnArgs turn) {
-  extern __shared__ int s_hist[];      // [n_adapters + 1], a turned tile
-  if ((int)blockIdx.x >= p.blocks) { turn_block(turn, blockIdx.x - p.blocks, s_hist); return; }
+__global__ void __launch_bounds__(1024) lowrank_plan_count_kernel(Plan p, Ids ids, PackArgs pack) {
+  extern __shared__ int s_hist[];      // [n_adapters + 1]
+  if ((int)blockIdx.x >= p.blocks) {
+    if (pack.es == 4) pack_block<uint32_t>(pack, blockIdx.x - p.blocks);
+    else pack_block<unsigned short>(pack, blockIdx.x - p.blocks);
+    return;
+  }
   for (int g = threadIdx.x; g <= p.n_adapters; g += 1024) s_hist[g] = 0;
   __syncthreads();
   const int first = blockIdx.x * p.block_rows, last = first + p.block_rows < p.rows ? first + p.block_rows : p.rows;
@@ -73,23 +101,28 @@ __global__ void __launch_bounds__(1024) lowrank_plan_count_kernel(Plan p, Ids id
   for (int g = threadIdx.x; g < p.n_adapters; g += 1024) p.hist[(int64_t)blockIdx.x * p.n_adapters + g] = s_hist[g];
 }
 struct PlanLds {      // of lowrank_plan_place_kernel: all [n_adapters + 2], next [16][n_adapters + 1]
-  int *first, *mine, *range0, *chunk0, *slot0, *next;
-  __host__ __device__ static size_t bytes(int G) { return (size_t)(5 * (G + 2) + 16 * (G + 1)) * 4; }
-  __device__ explicit PlanLds(int *s, int G) : first(s), mine(s + G + 2), range0(s + 2 * (G + 2)), chunk0(s + 3 * (G + 2)), slot0(s + 4 * (G + 2)), next(s + 5 * (G + 2)) {}
+  int *first, *mine, *range0, *wide0, *chunk0, *slot0, *next;
+  __host__ __device__ static size_t bytes(int G) { return (size_t)(6 * (G + 2) + 16 * (G + 1)) * 4; }
+  __device__ explicit PlanLds(int *s, int G) : first(s), mine(s + G + 2), range0(s + 2 * (G + 2)), wide0(s + 5 * (G + 2)), chunk0(s + 3 * (G + 2)), slot0(s + 4 * (G + 2)), next(s + 6 * (G + 2)) {}
 };
 __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids ids) {
   extern __shared__ int s_mem[];
-  __shared__ int s_w[16][3], s_all[1024], s_mine[1024], s_per;
+  __shared__ int s_w[16][4], s_all[1024], s_mine[1024], s_per;
   const int G = p.n_adapters, G1 = G + 1, t = threadIdx.x, lane = t & 63, wave = t >> 6, me = blockIdx.x;
   PlanLds s(s_mem, G);
+  // the share's rows: each wave owns a run of them, so that places follow the rows' order
+  const int first_row = me * p.block_rows, last_row = first_row + p.block_rows < p.rows ? first_row + p.block_rows : p.rows, run = p.block_rows / 16;
+  const int from = first_row + wave * run, to = from + run < last_row ? from + run : last_row;
+  const int h0 = from + lane < to ? group_of(ids, from + lane) : 0;      // (most shares have one row a lane: read once)
   for (int i = t; i < 16 * G1; i += 1024) s.next[i] = 0;
   if (t == 0) s_per = LR_RANGE;
   // the adapters' rows in all shares and in the shares before this one
-  int width = 1;
+  int width = 1, slices = 1;
   while (width < G) width <<= 1;
-  const int slices = 1024 / width, slice = t / width, g = t & (width - 1);
+  while (slices < p.blocks && slices * width < 1024) slices <<= 1;
+  const int slice = t / width, g = t & (width - 1);
   int all = 0, mine = 0;
-  if (g < G) {
+  if (g < G && slice < slices) {
 #pragma unroll 4
     for (int b = slice; b < p.blocks; b += slices) {
       const int c = p.hist[(int64_t)b * G + g];
@@ -97,50 +130,65 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     }
   }
   s_all[t] = all; s_mine[t] = mine;
-  // beside it, the share's rows by wave and group: each wave owns a run of rows, so that places follow the rows' order
-  const int first_row = me * p.block_rows, last_row = first_row + p.block_rows < p.rows ? first_row + p.block_rows : p.rows, run = p.block_rows / 16;
-  const int from = first_row + wave * run, to = from + run < last_row ? from + run : last_row;
   __syncthreads();
-  for (int i = from + lane; i < to; i += 64) atomicAdd(&s.next[wave * G1 + group_of(ids, i)], 1);
+  if (from + lane < to) atomicAdd(&s.next[wave * G1 + h0], 1);
+  for (int i = from + 64 + lane; i < to; i += 64) atomicAdd(&s.next[wave * G1 + group_of(ids, i)], 1);
   for (int h = slices >> 1; h > 0; h >>= 1) {
     if (slice < h) { s_all[t] += s_all[t + h * width]; s_mine[t] += s_mine[t + h * width]; }
     __syncthreads();
   }
-  int3 sum, at;
   const int n = t < G ? s_all[t] : 0, chunks = (n + LR_CHUNK - 1) / LR_CHUNK;
-  at = block_scan3({n, chunks, chunks > 1 ? chunks : 0}, &sum, s_w);
-  const int idle = p.rows - sum.x;
+  int at[4] = {n, chunks, chunks > 1 ? chunks : 0, t < G ? s_mine[t] : 0}, sum[4];
+  block_scan(at, sum, s_w);
+  const int idle = p.rows - sum[0];
   // the smallest size of a range that makes no more of them than are wanted: a wave tries a size
   for (int per = p.per + wave; per < LR_RANGE; per += 16) {
     int k = 0;
-    for (int i = lane; i < G; i += 64) k += (s_all[i] + per - 1) / per;
+    for (int i = lane; i < G; i += 64) k += (int)((unsigned)(s_all[i] + per - 1) / (unsigned)per);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) k += __shfl_xor(k, o);
-    if (lane == 0 && k + (idle + per - 1) / per <= p.wanted) atomicMin(&s_per, per);
+    k += (int)((unsigned)(idle + per - 1) / (unsigned)per);
+    if (k <= p.wanted) {      // sizes behind it make no more
+      if (lane == 0) atomicMin(&s_per, per);
+      break;
+    }
   }
-  if (t < G) { s.first[t] = at.x; s.chunk0[t] = at.y; s.slot0[t] = at.z; s.mine[t] = s_mine[t]; }
-  if (t == 0) { s.first[G] = sum.x; s.first[G + 1] = p.rows; s.chunk0[G] = sum.y; }
-  int3 msum;
-  const int3 unused = block_scan3({t < G ? s_mine[t] : 0, 0, 0}, &msum, s_w);
-  (void)unused;
-  if (t == 0) s.mine[G] = me * p.block_rows - msum.x;
-  const int per = s_per;      // (behind the scan's barriers)
-  int3 rsum;
-  const int3 rat = block_scan3({(n + per - 1) / per, 0, 0}, &rsum, s_w);
-  if (t < G) s.range0[t] = rat.x;
-  if (t == 0) { s.range0[G] = rsum.x; s.range0[G + 1] = rsum.x + (idle + per - 1) / per; }
-  if (t < G && me == 0) p.slots[t] = {at.z, chunks};
+  if (t < G) { s.first[t] = at[0]; s.chunk0[t] = at[1]; s.slot0[t] = at[2]; s.mine[t] = s_mine[t]; }
+  if (t == 0) { s.first[G] = sum[0]; s.first[G + 1] = p.rows; s.chunk0[G] = sum[1]; s.mine[G] = first_row - sum[3]; }
+  if (t < G && me == 0) p.slots[t] = {at[2], chunks};
+  __syncthreads();
+  const unsigned per = (unsigned)s_per;
+  int rat[2] = {(int)((unsigned)(n + per - 1) / per), (n + LR_WIDE - 1) / LR_WIDE}, rsum[2];
+  block_scan(rat, rsum, s_w);
+  if (t < G) { s.range0[t] = rat[0]; s.wide0[t] = rat[1]; }
+  if (t == 0) {
+    s.wide0[G] = rsum[1]; s.wide0[G + 1] = rsum[1] + (idle + LR_WIDE - 1) / LR_WIDE;
+    s.range0[G] = rsum[0]; s.range0[G + 1] = rsum[0] + (int)((unsigned)(idle + per - 1) / per);
+  }
+  // where each wave's rows of each group go: 16 lanes a group
+  for (int h = t >> 4; h < G1; h += 64) {
+    const int w = t & 15, c = s.next[w * G1 + h];
+    int i = c;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      const int u = __shfl_up(i, o, 16);
+      i += w >= o ? u : 0;
+    }
+    s.next[w * G1 + h] = s.first[h] + s.mine[h] + i - c;
+  }
   __syncthreads();
   const int step = gridDim.x * 1024, ranges = s.range0[G + 1], n_chunks = s.chunk0[G];
-  for (int i = me * 1024 + t; i < p.n_ranges; i += step) {      // the ranges of an adapter are of about one size
+  auto put = [&](int i, const int *range0, int count, int4 *out) {      // the ranges of an adapter are of about one size
     int4 r = {0, 0, 0, 0};
-    if (i < ranges) {
-      const int h = find_group(s.range0, G1, i), k = i - s.range0[h], m = s.range0[h + 1] - s.range0[h], rows = s.first[h + 1] - s.first[h];
-      const int a = (int)((int64_t)rows * k / m), b = (int)((int64_t)rows * (k + 1) / m);
-      r = {h, s.first[h] + a, b - a, 0};
+    if (i < count) {
+      const int h = find_group(range0, G1, i);
+      const unsigned k = i - range0[h], m = range0[h + 1] - range0[h], rows = s.first[h + 1] - s.first[h], size = rows / m, more = rows % m;
+      r = {h, s.first[h] + (int)(k * size + (k < more ? k : more)), (int)(size + (k < more ? 1u : 0u)), 0};
     }
-    p.range[i] = r;
-  }
+    out[i] = r;
+  };
+  for (int i = me * 1024 + t; i < p.n_ranges; i += step) put(i, s.range0, ranges, p.range);
+  for (int i = me * 1024 + t; i < p.n_wide; i += step) put(i, s.wide0, s.wide0[G1], p.wide);
   for (int i = me * 1024 + t; i < p.max_chunks; i += step) {
     int4 r = {0, 0, 0, -1};
     if (i < n_chunks) {      // the chunks of an adapter are of one size, whole steps of 32 rows
@@ -150,17 +198,11 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     }
     p.chunk[i] = r;
   }
-  for (int h = t; h < G1; h += 1024) {
-    int place = s.first[h] + s.mine[h];
-#pragma unroll 4
-    for (int w = 0; w < 16; ++w) { const int c = s.next[w * G1 + h]; s.next[w * G1 + h] = place; place += c; }
-  }
-  __syncthreads();
   int bits = 0;
   while ((1 << bits) < G1) ++bits;
   for (int i0 = from; i0 < to; i0 += 64) {
     const bool in = i0 + lane < to;
-    const int h = in ? group_of(ids, i0 + lane) : 0;
+    const int h = i0 == from ? h0 : in ? group_of(ids, i0 + lane) : 0;
     uint64_t same = __ballot(in);      // the lanes with my group
     for (int b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((h >> b) & 1);
@@ -178,10 +220,8 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
   }
 }
 
-void lowrank_plan_launch(const Plan &p, const Ids &ids, const TurnArgs &turn, hipStream_t stream) {
-  const unsigned turned = (unsigned)turn.blocks * (unsigned)p.n_adapters;
-  const size_t count = (size_t)(p.n_adapters + 1) * 4, tile = turned > 0 ? 64 * 65 * (size_t)turn.es : 0;
-  lowrank_plan_count_kernel<<<(unsigned)p.blocks + turned, 1024, count > tile ? count : tile, stream>>>(p, ids, turn);
+void lowrank_plan_launch(const Plan &p, const Ids &ids, const PackArgs &pack, hipStream_t stream) {
+  lowrank_plan_count_kernel<<<(unsigned)(p.blocks + pack.n_blocks), 1024, (size_t)(p.n_adapters + 1) * 4, stream>>>(p, ids, pack);
   lowrank_plan_place_kernel<<<p.blocks, 1024, PlanLds::bytes(p.n_adapters), stream>>>(p, ids);
 }
 
@@ -223,11 +263,13 @@ static void lowrank_layout(Lowrank *q, const gsdf_lowrank_args *a, void *save, v
   void *plan_saved = s.take<char>(plan_bytes);
   q->ht = s.take<float>(ht_bytes);
   const size_t weights = (size_t)a->n_adapters * q->rp * q->es, part = (size_t)plan_max_slots(a->rows, a->n_adapters) * q->rp * 4;
-  q->turned[0] = s.take<char>(weights * a->n_in);
-  q->turned[1] = s.take<char>(weights * a->n_out);
+  const int step = 128 / q->es;
+  q->a_turned = s.take<char>(weights * a->n_in);
+  q->b_frag = s.take<char>(weights * align_up((size_t)a->n_out, step));
   q->save_bytes = s.used;
   void *plan_ws = f.take<char>(plan_bytes);
   q->h = f.take<float>(h_bytes);
+  q->a_frag = f.take<char>(weights * align_up((size_t)a->n_in, step));
   q->fwd_ws_bytes = f.used;      // the plan at least: never 0
   plan_layout(&q->plan, training ? plan_saved : plan_ws, a->rows, a->n_adapters, least);
   q->dh = b.take<float>(h_bytes);
@@ -237,16 +279,19 @@ static void lowrank_layout(Lowrank *q, const gsdf_lowrank_args *a, void *save, v
   q->bwd_ws_bytes = b.used > 0 ? b.used : 256;      // (a buffer that a caller can point to)
 }
 
-TurnArgs lowrank_turn_args(const Lowrank &q, bool training) {
+PackArgs lowrank_pack_args(const Lowrank &q, bool training) {
   const gsdf_lowrank_args &a = q.a;
-  TurnArgs t;
-  t.in[0] = a.a; t.out[0] = q.turned[0]; t.rows[0] = a.rank; t.cols[0] = a.n_in; t.out_ld[0] = q.rp;
-  t.in[1] = a.b; t.out[1] = q.turned[1]; t.rows[1] = a.n_out; t.cols[1] = a.rank; t.out_ld[1] = a.n_out;
-  t.blocks0 = (int)(ceil_div(q.rp, 64) * ceil_div(a.n_in, 64));
-  t.blocks = training && a.rows > 0 ? t.blocks0 + (int)(ceil_div(a.n_out, 64) * ceil_div(a.rank, 64)) : 0;
-  t.es = q.es;
+  const int step = 128 / q.es;
+  PackArgs t;
+  t.a = a.a; t.b = a.b; t.a_frag = q.a_frag; t.b_frag = q.b_frag; t.a_turned = q.a_turned;
+  t.n_in = a.n_in; t.n_out = a.n_out; t.rank = a.rank; t.rt = q.rt; t.es = q.es;
+  t.blocks[0] = (int)ceil_div(ceil_div(a.n_in, step) * q.rt * 128, 1024);
+  t.blocks[1] = training ? (int)ceil_div(ceil_div(a.n_out, step) * q.rt * 128, 1024) : 0;
+  t.blocks[2] = training ? (int)ceil_div((int64_t)a.n_in * q.rp / (16 / q.es), 1024) : 0;
+  t.n_blocks = a.rows > 0 ? (t.blocks[0] + t.blocks[1] + t.blocks[2]) * a.n_adapters : 0;
   return t;
 }
+
 }  // namespace gsdf
 
 extern "C" size_t gsdf_lowrank_save_bytes(const gsdf_lowrank_args *a) {
@@ -282,7 +327,7 @@ extern "C" int gsdf_lowrank_fwd(const gsdf_lowrank_args *args, const void *base,
   Lowrank q;
   lowrank_layout(&q, args, save, ws, save != nullptr);
   if (args->rows == 0) {      // the backward pass asks the plan which adapters have rows
-    lowrank_plan_launch(q.plan, Ids{args->ids, args->ids_64, args->n_adapters}, lowrank_turn_args(q, false), stream);
+    lowrank_plan_launch(q.plan, Ids{args->ids, args->ids_64, args->n_adapters}, lowrank_pack_args(q, false), stream);
   } else {
     GSDF_BY_DTYPE(args->dtype, lowrank_fwd<T>(q, base, base_stride, y, y_stride, save != nullptr, stream));
   }

@@ -116,8 +116,8 @@ __device__ __forceinline__ float scale_to_one(float largest) {
 // RT: tiles of 16 ranks.  H: [places][16 RT] (for `expand`) and / or HT: [16 RT][ht_ld] (for `outer`), zeros behind the rank.
 struct ShrinkArgs {
   const void *x, *w;
-  int64_t x_stride, w_group;      // elements between rows; between the adapters' matrices
-  int width, w_ld, rank, split;
+  int64_t x_stride;               // elements between rows
+  int width, rank, split;         // w: fragments (PackArgs)
   const float *scales;            // per adapter, or null
   float factor;
   float *h, *ht;
@@ -144,26 +144,23 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
     row[t] = (uint32_t)q.plan.order[range.y + (i < range.z ? i : range.z - 1)];
     px[t] = (const T *)q.x + (int64_t)row[t] * q.x_stride;
   }
-  const T *pw[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int j = r * 16 + c;
-    pw[r] = (const T *)q.w + range.x * q.w_group + (int64_t)(j < q.rank ? j : q.rank - 1) * q.w_ld;
-  }
+  const V *pw = (const V *)q.w + (int64_t)range.x * ((q.width + STEP - 1) / STEP) * RT * 128 + lane;
   // Ranges begin at different steps: rows of 2^n bytes at the same step would all ask the same memory channels (19 against 15 us for 64 MB).
   const int full = q.width / STEP, turn = full > 0 ? (int)((unsigned)which % (unsigned)full) : 0;
-  auto column = [&](int step) { return (step + turn < full ? step + turn : step + turn - full) * STEP + quad * N; };
-  auto load = [&](int k, V (&xs)[TT][2], V (&ws)[RT][2]) {
+  auto place = [&](int step) { return step + turn < full ? step + turn : step + turn - full; };
+  auto load = [&](int step, V (&xs)[TT][2], V (&ws)[RT][2]) {
+    const int k = step * STEP + quad * N;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int t = 0; t < TT; ++t) xs[t][i] = load_vec<T>(px[t] + k + i * 4 * N);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) ws[r][i] = load_vec<T>(pw[r] + k + i * 4 * N);
+      for (int r = 0; r < RT; ++r) ws[r][i] = pw[((int64_t)step * RT + r) * 128 + i * 64];
     }
   };
-  auto add = [&](int k, V (&xs)[TT][2], V (&ws)[RT][2]) {
+  auto add = [&](int step, V (&xs)[TT][2], V (&ws)[RT][2]) {
     if (DROP) {
+      const int k = step * STEP + quad * N;
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -181,16 +178,16 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
   for (; s + (AHEAD - 1) * q.split < full; s += AHEAD * q.split) {
     V xs[AHEAD][TT][2], ws[AHEAD][RT][2];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) load(column(s + u * q.split), xs[u], ws[u]);
+    for (int u = 0; u < AHEAD; ++u) load(place(s + u * q.split), xs[u], ws[u]);
     __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler saves registers and lets two loads go at a time)
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) add(column(s + u * q.split), xs[u], ws[u]);
+    for (int u = 0; u < AHEAD; ++u) add(place(s + u * q.split), xs[u], ws[u]);
   }
   for (; s < full; s += q.split) {
     V xs[TT][2], ws[RT][2];
-    load(column(s), xs, ws);
+    load(place(s), xs, ws);
     __builtin_amdgcn_sched_barrier(0);
-    add(column(s), xs, ws);
+    add(place(s), xs, ws);
   }
   if (RAGGED && part == full % q.split) {      // the rows' last elements
     const int k = full * STEP + quad * N;
@@ -198,11 +195,11 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) xs[t][i] = load_vec_end<T>(px[t], k + i * 4 * N, q.width);
+      for (int r = 0; r < RT; ++r) ws[r][i] = pw[((int64_t)full * RT + r) * 128 + i * 64];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) ws[r][i] = load_vec_end<T>(pw[r], k + i * 4 * N, q.width);
+      for (int t = 0; t < TT; ++t) xs[t][i] = load_vec_end<T>(px[t], k + i * 4 * N, q.width);
     }
-    add(k, xs, ws);
+    add(full, xs, ws);
   }
   const float f = q.factor * (q.scales != nullptr ? q.scales[range.x] : 1.f);
   auto put = [&](int r, int t, f32x4 v) {
@@ -252,65 +249,82 @@ __global__ void __launch_bounds__(512) lowrank_shrink_kernel(ShrinkArgs q) {
 }
 
 // ---- expand: y[row][n] = base[row][n] + sum_j H[place][j] W[g][n][j] -------------------------------------------------------------------------
-// A wave takes 64 columns of a tile at a time: four matrix tiles whose rows are columns of y in the order that
-// leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of them.
+// A wave takes 64 columns of up to 64 rows (the weights come from the L2, whose bandwidth bounds the wider ranks: 32 rows a read took 40 us for a rank of 64
+// where 64 take 3x).  The instruction's rows are columns of y in the order that leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of
+// them; lanes of rows c and c + 8 then change pieces, so that an access covers 128 bytes of each of 8 rows instead of 64 of 16 (30 against 34 us for
+// a plain copy of 8192 rows of 8 KB in this manner).
 struct ExpandArgs {
   const float *h;
   const void *w, *base;
   void *y;
   int64_t w_group, base_stride, y_stride;
-  int width, w_ld, rank;
-  bool past;         // y goes past the caches
+  int width, w_ld, rank, parts;      // parts: waves that share a range's columns
   Dropout drop;      // on the result (dx), DROP only
   Plan plan;
 };
-template <typename T, int RT, int TT, bool DROP, bool RAGGED>
-__device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int turn, int chunks) {
-  typedef typename Vec<T>::vec V;
-  constexpr int N = Vec<T>::N, NB = 16 / N;      // pieces of a lane's 16 columns: piece p at column 4 N p + N quad of the 64
-  constexpr bool WIDE = sizeof(T) == 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
-  const bool idle = range.x == q.plan.n_adapters;
-  if (idle && q.base == q.y) return;      // in place: not touched
-  int64_t row[TT];
-  bool mine[TT];
+// lanes c and c + 8 of each 16: a of the lower and b of the upper one stay, the lower one's b and the upper one's a change places.  Its own inverse.
+template <typename V>
+__device__ __forceinline__ void change_halves(V &a_, V &b_, bool upper) {
+  u32x4 a = __builtin_bit_cast(u32x4, a_), b = __builtin_bit_cast(u32x4, b_);
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    const int i = t * 16 + c;
-    mine[t] = i < range.z;
-    row[t] = q.plan.order[range.y + (mine[t] ? i : range.z - 1)];
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t away = upper ? a[i] : b[i], come = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)away, 0x128, 0xF, 0xF, true);      // row_ror:8
+    a[i] = upper ? come : a[i];
+    b[i] = upper ? b[i] : come;
   }
-  const T *base = (const T *)q.base;
-  T *y = (T *)q.y;
-  auto store = [&](T *p, int valid, const float (&v)[N]) {
-    if (!RAGGED || valid >= N) {
-      V o;
+  a_ = __builtin_bit_cast(V, a);
+  b_ = __builtin_bit_cast(V, b);
+}
+template <typename T, int RT, int TT, bool DROP, bool RAGGED, bool PAST>
+__device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int part, int turn, int chunks) {
+  typedef typename Vec<T>::vec V;
+  constexpr int N = Vec<T>::N, NP = 8 / N;      // pairs of pieces of a lane's 16 columns: piece p at column 4 N p + N quad of the 64
+  constexpr bool WIDE = sizeof(T) == 4;
+  const int lane = threadIdx.x & 63, c = lane & 15, quad = lane >> 4;
+  const bool upper = c >= 8, idle = range.x == q.plan.n_adapters, add = q.base != nullptr;
+  const int *order = q.plan.order + range.y;
+  // access 2 t + half: rows 16 t + 8 half + c % 8, the lower lanes their first 64 bytes of a pair, the upper ones the second
+  const T *base[2 * TT];
+  T *y[2 * TT];
+  const int column = (upper ? 4 * N : 0) + quad * N;
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = (T)v[e];
-      if (q.past) __builtin_nontemporal_store(o, reinterpret_cast<typename Piece<T, N>::any *>(p));
-      else *reinterpret_cast<typename Piece<T, N>::any *>(p) = o;
+  for (int i = 0; i < 2 * TT; ++i) {
+    const int at = i * 8 + (c & 7);
+    const int64_t row = order[at < range.z ? at : range.z - 1];
+    base[i] = (const T *)q.base + row * q.base_stride;
+    y[i] = (T *)q.y + row * q.y_stride;
+  }
+  auto load_base = [&](int ch, V (&b)[2 * TT][NP]) {
+#pragma unroll
+    for (int i = 0; i < 2 * TT; ++i)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int n = ch * 64 + p * 8 * N + column;
+        if (!add) b[i][p] = V{};
+        else if (!RAGGED || n + N <= q.width) b[i][p] = load_vec<T>(base[i] + n);
+        else b[i][p] = load_vec_end<T>(base[i], n, q.width);
+      }
+  };
+  auto store = [&](int i, int n, V v) {
+    if (i * 8 + (c & 7) >= range.z) return;
+    if (!RAGGED || n + N <= q.width) {
+      if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename Piece<T, N>::any *>(y[i] + n));
+      else *reinterpret_cast<typename Piece<T, N>::any *>(y[i] + n) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (e < valid) p[e] = (T)v[e];
+        if (n + e < q.width) y[i][n + e] = v[e];
     }
   };
   if (idle) {
-    for (int i = blockIdx.y * 4 + wave; i < chunks; i += gridDim.y * 4) {
+    for (int i = part; i < chunks; i += q.parts) {
       const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
+      V b[2 * TT][NP];
+      load_base(ch, b);
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
+      for (int r = 0; r < 2 * TT; ++r)
 #pragma unroll
-        for (int p = 0; p < NB; ++p) {
-          const int n = ch * 64 + p * 4 * N + quad * N;
-          if ((RAGGED && n >= q.width) || !mine[t]) continue;
-          float v[N];
-          V b;
-          if (base != nullptr) b = !RAGGED || n + N <= q.width ? load_vec<T>(base + row[t] * q.base_stride + n) : load_vec_end<T>(base + row[t] * q.base_stride, n, q.width);
-#pragma unroll
-          for (int e = 0; e < N; ++e) v[e] = base != nullptr ? (float)b[e] : 0.f;
-          store(y + row[t] * q.y_stride + n, q.width - n, v);
-        }
+        for (int p = 0; p < NP; ++p) store(r, ch * 64 + p * 8 * N + column, b[r][p]);
     }
     return;
   }
@@ -320,20 +334,23 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
   constexpr int KB = WIDE ? RT : (RT == 1 ? 1 : RT / 2);
   V hi[TT][KB], lo[TT][KB];
   float back[TT];
+  uint32_t row_of[TT];
   auto rank_of = [&](int k) { return WIDE ? k * 16 + quad * 4 : (RT == 1 ? (quad & 1) * 8 : k * 32 + quad * 8); };
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const float *ph = q.h + (int64_t)(range.y + (mine[t] ? t * 16 + c : range.z - 1)) * (16 * RT);
+    const int at = t * 16 + c < range.z ? t * 16 + c : range.z - 1;
+    if (DROP) row_of[t] = (uint32_t)order[at];
+    const float *ph = q.h + (int64_t)(range.y + at) * (16 * RT);
     f32x4 f[KB][N / 4];
     float largest = 0.f;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        f[k][i] = *reinterpret_cast<const f32x4 *>(ph + rank_of(k) + i * 4);
-        if (DROP) f[k][i] *= q.drop.scale;
+      for (int e = 0; e < N / 4; ++e) {
+        f[k][e] = *reinterpret_cast<const f32x4 *>(ph + rank_of(k) + e * 4);
+        if (DROP) f[k][e] *= q.drop.scale;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(f[k][i][e]));
+        for (int l = 0; l < 4; ++l) largest = fmaxf(largest, fabsf(f[k][e][l]));
       }
     float down = 1.f;
     back[t] = 1.f;
@@ -346,94 +363,90 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float v = f[k][i / 4][i % 4] * down;
+      for (int e = 0; e < N; ++e) {
+        const float v = f[k][e / 4][e % 4] * down;
         const T h = (T)v;
         const T l = (T)(v - (float)h);
-        hi[t][k][i] = !WIDE && RT == 1 && quad >= 2 ? l : h;
-        lo[t][k][i] = l;
+        hi[t][k][e] = !WIDE && RT == 1 && quad >= 2 ? l : h;
+        lo[t][k][e] = l;
       }
   }
-  auto body = [&](int ch, auto columns_whole, auto ranks_whole) {
-    const int n0 = ch * 64 + quad * N;
-    V b[TT][NB], u[4][KB];
+  for (int i = part; i < chunks; i += q.parts) {
+    const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
+    const bool whole = !RAGGED || (ch * 64 + 64 <= q.width && q.rank % N == 0);
+    V b[2 * TT][NP], u[4][KB];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       const int col = ch * 64 + m * 4 / N * 4 * N + (c >> 2) * N + m * 4 % N + (c & 3);      // the column that this lane's weights belong to
-      const T *pw = w + (int64_t)(columns_whole || col < q.width ? col : q.width - 1) * q.w_ld;
+      const T *pw = w + (int64_t)(whole || col < q.width ? col : q.width - 1) * q.w_ld;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
         const int j = rank_of(k);
-        if (ranks_whole) u[m][k] = load_vec<T>(pw + (j < q.rank ? j : 0));
+        if (whole) u[m][k] = load_vec<T>(pw + (j < q.rank ? j : 0));
         else u[m][k] = load_vec_end<T>(pw, j, q.rank);
       }
     }
-    if (base != nullptr) {
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int p = 0; p < NB; ++p)
-          b[t][p] = columns_whole ? load_vec<T>(base + row[t] * q.base_stride + n0 + p * 4 * N)
-                                  : load_vec_end<T>(base + row[t] * q.base_stride, n0 + p * 4 * N, q.width);
-    }
+    load_base(ch, b);
     __builtin_amdgcn_sched_barrier(0);
-    float v[TT][16];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      f32x4 acc[TT];
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-      for (int t = 0; t < TT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        if (ranks_whole) u[m][k] = zero_unless<T>(rank_of(k) < q.rank, u[m][k]);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          acc[t] = mma(u[m][k], hi[t][k], acc[t]);
-          if (!WIDE && RT > 1) acc[t] = mma(u[m][k], lo[t][k], acc[t]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[t][m * 4 + e] = acc[t][e];
-    }
+      for (int k = 0; k < KB; ++k) u[m][k] = zero_unless<T>(rank_of(k) < q.rank, u[m][k]);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      if (!mine[t]) continue;
+      f32x4 acc[4];
 #pragma unroll
-      for (int p = 0; p < NB; ++p) {
-        const int n = n0 + p * 4 * N;
-        float o[N];
+      for (int m = 0; m < 4; ++m) {
+        acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = v[t][p * N + e] * back[t] + (base != nullptr ? (float)b[t][p][e] : 0.f);
-        if (DROP) {
-          uint32_t bits[4];
-          dropout_bits(q.drop, (uint32_t)n >> 3, (uint32_t)row[t], bits);
-          if (N == 4 && (n & 4)) { bits[0] = bits[2]; bits[1] = bits[3]; }
-#pragma unroll
-          for (int e = 0; e < N; ++e) o[e] = dropout_keeps(q.drop, bits, e) ? o[e] : 0.f;
+        for (int k = 0; k < KB; ++k) {
+          acc[m] = mma(u[m][k], hi[t][k], acc[m]);
+          if (!WIDE && RT > 1) acc[m] = mma(u[m][k], lo[t][k], acc[m]);
         }
-        store(y + row[t] * q.y_stride + n, columns_whole ? N : q.width - n, o);
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        V o[2];
+        if (add) change_halves(b[2 * t][p], b[2 * t + 1][p], upper);      // now the pieces 2 p and 2 p + 1 of the lane's own row
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int piece = 2 * p + s, n = ch * 64 + piece * 4 * N + quad * N;
+          float v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            v[e] = acc[(piece * N + e) / 4][e % 4] * back[t];
+            if (add) v[e] += (float)b[2 * t + s][p][e];
+          }
+          if (DROP) {
+            uint32_t bits[4];
+            dropout_bits(q.drop, (uint32_t)n >> 3, row_of[t], bits);
+            if (N == 4 && (n & 4)) { bits[0] = bits[2]; bits[1] = bits[3]; }
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = dropout_keeps(q.drop, bits, e) ? v[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[s][e] = (T)v[e];
+        }
+        change_halves(o[0], o[1], upper);
+        store(2 * t, ch * 64 + p * 8 * N + column, o[0]);
+        store(2 * t + 1, ch * 64 + p * 8 * N + column, o[1]);
       }
     }
-  };
-  for (int i = blockIdx.y * 4 + wave; i < chunks; i += gridDim.y * 4) {
-    const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
-    if (!RAGGED) body(ch, std::true_type{}, std::true_type{});
-    else if (ch * 64 + 64 <= q.width && q.rank % N == 0) body(ch, std::true_type{}, std::true_type{});
-    else body(ch, std::false_type{}, std::false_type{});
   }
 }
-template <typename T, int RT, bool DROP, bool RAGGED>      // RAGGED: the width is no multiple of 64 or the rank none of a lane's piece
-__global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT == 4 ? 3 : 2) lowrank_expand_kernel(ExpandArgs q) {
-  const int4 range = q.plan.range[blockIdx.x];
-  if (range.z == 0) return;
-  const int chunks = (q.width + 63) / 64;
-  const int turn = (int)(blockIdx.x % (unsigned)chunks);      // ranges begin at different columns: not all at the same memory channels
+// RAGGED: the width is no multiple of 64 or the rank none of a lane's piece; PAST: y goes past the caches
+template <typename T, int RT, bool DROP, bool RAGGED, bool PAST>
+__global__ void __launch_bounds__(256, RAGGED || RT == 8 ? 1 : 2) lowrank_expand_kernel(ExpandArgs q) {
+  const unsigned id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), which = id / (unsigned)q.parts;
+  if (which >= (unsigned)q.plan.n_wide) return;
+  const int4 range = q.plan.wide[which];
+  if (range.z == 0 || (range.x == q.plan.n_adapters && q.base == q.y)) return;      // (in place a row without an adapter is not touched)
+  const int chunks = (q.width + 63) / 64, part = (int)(id % (unsigned)q.parts);
+  const int turn = (int)(which % (unsigned)chunks);      // ranges begin at different columns: not all at the same memory channels
   if (DROP) dropout_counter(q.drop);
-  if (range.z > 32) expand_range<T, RT, 3, DROP, RAGGED>(q, range, turn, chunks);
-  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED>(q, range, turn, chunks);
-  else expand_range<T, RT, 1, DROP, RAGGED>(q, range, turn, chunks);
+  if (range.z > 32) expand_range<T, RT, 4, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
+  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
+  else expand_range<T, RT, 1, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
 }
 
 // ---- outer: sum over an adapter's rows of UT[j][place] V[row][c] ----------------------------------------------------------------------------
@@ -701,6 +714,7 @@ __global__ void __launch_bounds__(256) lowrank_row_expand_kernel(Ids ids, const 
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------------
+// without gradients: so few rows that an adapter's weights are hardly read twice take no plan
 static constexpr int64_t LR_FEW_ROWS = 64;
 static constexpr int64_t LR_PAST = 32 << 20;      // bytes of a result from which on it is written past the caches
 
@@ -713,10 +727,9 @@ static constexpr int64_t LR_PAST = 32 << 20;      // bytes of a result from whic
   }
 
 template <typename T>
-static void shrink_launch(const Lowrank &q, const void *x, int64_t x_stride, int width, const void *w, int64_t w_group, int w_ld, const float *scales, bool drop, float *h,
-                          float *ht, hipStream_t stream) {
+static void shrink_launch(const Lowrank &q, const void *x, int64_t x_stride, int width, const void *w, const float *scales, bool drop, float *h, float *ht, hipStream_t stream) {
   ShrinkArgs s;
-  s.x = x; s.w = w; s.x_stride = x_stride; s.w_group = w_group; s.width = width; s.w_ld = w_ld; s.rank = q.a.rank;
+  s.x = x; s.w = w; s.x_stride = x_stride; s.width = width; s.rank = q.a.rank;
   s.scales = scales; s.factor = drop ? q.drop.scale : 1.f; s.h = h; s.ht = ht; s.ht_ld = q.ht_ld; s.drop = q.drop; s.plan = q.plan;
   const int steps = (int)ceil_div(width, 128 / (int)sizeof(T));
   s.split = steps >= 8 ? 8 : steps >= 4 ? 4 : steps >= 2 ? 2 : 1;
@@ -736,15 +749,21 @@ static void expand_launch(const Lowrank &q, const float *h, const void *w, int64
   ExpandArgs s;
   s.h = h; s.w = w; s.base = base; s.y = y; s.w_group = w_group; s.base_stride = base_stride; s.y_stride = y_stride; s.width = width; s.w_ld = w_ld; s.rank = ranks;
   s.drop = q.drop; s.plan = q.plan;
-  s.past = (int64_t)q.a.rows * width * (int64_t)sizeof(T) >= LR_PAST;
   const int64_t chunks = ceil_div(width, 64);
-  const dim3 grid((unsigned)q.plan.n_ranges, (unsigned)ceil_div(chunks, chunks >= 16 ? 16 : 4));
-  const bool ragged = width % 64 != 0 || ranks % (16 / (int)sizeof(T)) != 0;
+  // one chunk of 64 columns a wave until there are more than eight waves a SIMD, then more
+  s.parts = (int)ceil_div(chunks, ceil_div(chunks * q.plan.n_wide, LR_CUS * 4 * 8));
+  const unsigned grid = (unsigned)ceil_div((int64_t)q.plan.n_wide * s.parts, 4);
+  const bool ragged = width % 64 != 0 || ranks % (16 / (int)sizeof(T)) != 0, past = (int64_t)q.a.rows * width * (int64_t)sizeof(T) >= LR_PAST;
+  auto run = [&](auto rt, auto drop_) {
+    constexpr int RT = decltype(rt)::value;
+    constexpr bool DROP = decltype(drop_)::value;
+    if (ragged) lowrank_expand_kernel<T, RT, DROP, true, false><<<grid, 256, 0, stream>>>(s);
+    else if (past) lowrank_expand_kernel<T, RT, DROP, false, true><<<grid, 256, 0, stream>>>(s);
+    else lowrank_expand_kernel<T, RT, DROP, false, false><<<grid, 256, 0, stream>>>(s);
+  };
   GSDF_BY_RANK(q.rt, {
-    if (drop && ragged) lowrank_expand_kernel<T, RT, true, true><<<grid, 256, 0, stream>>>(s);
-    else if (drop) lowrank_expand_kernel<T, RT, true, false><<<grid, 256, 0, stream>>>(s);
-    else if (ragged) lowrank_expand_kernel<T, RT, false, true><<<grid, 256, 0, stream>>>(s);
-    else lowrank_expand_kernel<T, RT, false, false><<<grid, 256, 0, stream>>>(s);
+    if (drop) run(std::integral_constant<int, RT>{}, std::true_type{});
+    else run(std::integral_constant<int, RT>{}, std::false_type{});
   });
 }
 
@@ -752,7 +771,7 @@ template <typename T>
 void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *y, int64_t y_stride, bool training, hipStream_t stream) {
   const gsdf_lowrank_args &a = q.a;
   const Ids ids = {a.ids, a.ids_64, a.n_adapters};
-  if (!training && a.rows <= LR_FEW_ROWS) {
+  if (!training && (a.rows <= LR_FEW_ROWS || a.rows <= 4 * (int64_t)a.n_adapters)) {
     lowrank_row_shrink_kernel<T><<<dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, 16)), 1024, 0, stream>>>(ids, (const T *)a.x, a.x_stride, (const T *)a.a, a.n_in, a.rank,
                                                                                                          a.scales, q.drop, q.h);
     lowrank_row_expand_kernel<T><<<dim3((unsigned)a.rows, (unsigned)(ceil_div(a.n_out, 64) < 4096 ? ceil_div(a.n_out, 64) : 4096)), 256, 0, stream>>>(
@@ -760,8 +779,8 @@ void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *
                                                                                                          base_stride, (T *)y, y_stride);
     return;
   }
-  lowrank_plan_launch(q.plan, ids, lowrank_turn_args(q, training), stream);
-  shrink_launch<T>(q, a.x, a.x_stride, a.n_in, a.a, (int64_t)a.rank * a.n_in, a.n_in, a.scales, q.drop.threshold != 0, q.h, training ? q.ht : nullptr, stream);
+  lowrank_plan_launch(q.plan, ids, lowrank_pack_args(q, training), stream);
+  shrink_launch<T>(q, a.x, a.x_stride, a.n_in, q.a_frag, a.scales, q.drop.threshold != 0, q.h, training ? q.ht : nullptr, stream);
   expand_launch<T>(q, q.h, a.b, (int64_t)a.n_out * a.rank, a.rank, a.rank, a.n_out, base, base_stride, y, y_stride, false, stream);
 }
 
@@ -771,9 +790,9 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
   const bool drop = q.drop.threshold != 0;
   const unsigned G = (unsigned)a.n_adapters;
   if (a.rows > 0 && (dx != nullptr || da != nullptr))
-    shrink_launch<T>(q, dy, dy_stride, a.n_out, q.turned[1], (int64_t)a.rank * a.n_out, a.n_out, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr, stream);
+    shrink_launch<T>(q, dy, dy_stride, a.n_out, q.b_frag, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr, stream);
   if (a.rows > 0 && dx != nullptr)
-    expand_launch<T>(q, q.dh, q.turned[0], (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride, drop, stream);
+    expand_launch<T>(q, q.dh, q.a_turned, (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride, drop, stream);
   if (da == nullptr && db == nullptr) return;
   constexpr int COLS = 16 * (16 / (int)sizeof(T));
   OuterArgs o;
