@@ -33,17 +33,49 @@ template <typename T>
 __device__ __forceinline__ typename Vec<T>::vec load_vec(const T *__restrict__ p) {
   return *reinterpret_cast<const typename Piece<T, Vec<T>::N>::any *>(p);
 }
-// the elements of a row from k on, 0 behind its end.  There every lane reads its row's first element instead of what is not there: no branch to each
-// element, and the loads leave together.
+// v moved down by n elements (0 .. N), zeros behind
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::vec move_down(typename Vec<T>::vec v, int n) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  u64x2 u = __builtin_bit_cast(u64x2, v);
+  const int bits = n * 8 * (int)sizeof(T), in = bits & 63;
+  const uint64_t low = bits >= 128 ? 0 : bits >= 64 ? u[1] : u[0], high = bits >= 64 ? 0 : u[1];
+  u[0] = (low >> in) | ((high << 1) << (63 - in));
+  u[1] = high >> in;
+  return __builtin_bit_cast(typename Vec<T>::vec, u);
+}
+// the elements of a row from k on, 0 behind its end: the row's last 16 bytes, moved down (one element after the other took a kernel from 8 to 18 us)
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::vec load_vec_end(const T *__restrict__ row, int k, int width) {
   constexpr int N = Vec<T>::N;
-  typename Vec<T>::vec v;
+  if (width >= N) {
+    const int at = k + N <= width ? k : width - N, by = k - at;
+    return move_down<T>(load_vec<T>(row + at), by < N ? by : N);
+  }
+  typename Vec<T>::vec v;      // a row of less than 16 bytes
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = row[k + i < width ? k + i : 0];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = k + i < width ? v[i] : (T)0.f;
   return v;
+}
+// the first `valid` (less than all) elements of v: by halves
+template <typename T>
+__device__ __forceinline__ void store_vec_end(T *p, int valid, typename Vec<T>::vec v) {
+  constexpr int N = Vec<T>::N;
+  if (N == 8 && (valid & 4)) {
+    typename Piece<T, 4>::vec t = {v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<typename Piece<T, 4>::any *>(p) = t;
+    v = move_down<T>(v, 4);
+    p += 4;
+  }
+  if (valid & 2) {
+    typename Piece<T, 2>::vec t = {v[0], v[1]};
+    *reinterpret_cast<typename Piece<T, 2>::any *>(p) = t;
+    v = move_down<T>(v, 2);
+    p += 2;
+  }
+  if (valid & 1) p[0] = v[0];
 }
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::vec zero_unless(bool keep, typename Vec<T>::vec v) {
@@ -52,22 +84,27 @@ __device__ __forceinline__ typename Vec<T>::vec zero_unless(bool keep, typename 
   for (int i = 0; i < 4; ++i) u[i] = keep ? u[i] : 0u;
   return __builtin_bit_cast(typename Vec<T>::vec, u);
 }
-// N (a multiple of 4) neighbouring results, `valid` of them
+// N (4, or 16 bytes) neighbouring results, `valid` of them
 template <typename T, int N>
 __device__ __forceinline__ void store_some(T *__restrict__ p, int valid, const float (&v)[N]) {
-  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
-  if (valid >= N) {
+  if constexpr (N == Vec<T>::N) {
+    typename Vec<T>::vec o;
 #pragma unroll
-    for (int i = 0; i < N; i += W) {
-      T t[W];
-#pragma unroll
-      for (int j = 0; j < W; ++j) t[j] = (T)v[i + j];
-      store_piece<T, W>(p + i, t);
-    }
+    for (int i = 0; i < N; ++i) o[i] = (T)v[i];
+    if (valid >= N) *reinterpret_cast<typename Piece<T, N>::any *>(p) = o;
+    else if (valid > 0) store_vec_end<T>(p, valid, o);
   } else {
+    if (valid >= N) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < valid) p[i] = (T)v[i];
+      for (int i = 0; i < N; i += 4) {
+        const T t[4] = {(T)v[i], (T)v[i + 1], (T)v[i + 2], (T)v[i + 3]};
+        store_piece<T, 4>(p + i, t);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < valid) p[i] = (T)v[i];
+    }
   }
 }
 // all ones in the half word (16-bit elements) of each element that stays: sat(bits - (threshold - 1)) is 0 exactly below the threshold
@@ -310,10 +347,8 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
     if (!RAGGED || n + N <= q.width) {
       if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename Piece<T, N>::any *>(y[i] + n));
       else *reinterpret_cast<typename Piece<T, N>::any *>(y[i] + n) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (n + e < q.width) y[i][n + e] = v[e];
+    } else if (n < q.width) {
+      store_vec_end<T>(y[i] + n, q.width - n, v);
     }
   };
   if (idle) {

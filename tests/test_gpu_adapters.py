@@ -36,7 +36,7 @@ SHAPES = [(1, 64, 64, 16, 1, 0.0, False), (1, 1, 1, 1, 1, 0.0, False), (2, 7, 5,
           (17, 129, 65, 17, 5, 0.0, False), (63, 200, 100, 64, 7, 0.2, True), (64, 256, 128, 32, 2, 0.0, True), (65, 72, 80, 128, 3, 0.0, False),
           (130, 1000, 1001, 12, 40, 0.1, False), (257, 40, 24, 100, 2, 0.5, False), (700, 136, 264, 16, 6, 0.05, False), (2500, 64, 64, 8, 6, 0.0, False),
           (5000, 32, 16, 4, 12, 0.1, True), (1500, 512, 96, 48, 9, 0.0, True), (3000, 16, 300, 20, 1000, 0.1, False), (900, 300, 16, 65, 1, 0.0, False),
-          (20000, 24, 40, 16, 9, 0.05, False), (40000, 8, 8, 2, 1024, 0.1, False), (4500, 264, 136, 96, 3, 0.0, True)]
+          (20000, 24, 40, 16, 9, 0.05, False), (40000, 8, 8, 2, 1024, 0.1, False), (70000, 64, 64, 8, 6, 0.05, False), (66000, 24, 72, 20, 5, 0.1, True), (65600, 72, 8, 4, 3, 0.0, False), (4500, 264, 136, 96, 3, 0.0, True)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
