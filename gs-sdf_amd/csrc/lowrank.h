@@ -7,7 +7,7 @@ namespace gsdf {
 static constexpr int LR_CUS = 256;          // compute units the ranges are dealt to
 static constexpr int LR_AIM = 40;           // rows of a range that are aimed at, at most
 static constexpr int LR_RANGE = 48;         // most rows of a range: three matrix tiles
-static constexpr int LR_WIDE = 64;           // most rows of a range of `expand`
+static constexpr int LR_BOTH = 65536;        // rows from which on a wave takes a range through both products
 static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
 
 // ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------
@@ -15,17 +15,17 @@ static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
 struct Plan {
   int *order;      // [rows]: the row at each place, adapters one behind the other, rows of one adapter in their own order
   int4 *range;     // [n_ranges]: adapter, first place, rows (0: unused), -
-  int4 *wide;      // [n_wide]: the same of up to LR_WIDE rows
+  int4 *wide;      // [n_wide]: the same of up to wide_rows rows, for `expand`
   int4 *chunk;     // [max_chunks]: adapter, first place, rows (0: unused), slot of its partial sums (-1: the adapter's only chunk)
   int2 *slots;     // [n_adapters]: first slot, chunks
   int *hist;       // [blocks][n_adapters]: rows of each adapter in each workgroup's share
   int rows, n_adapters, blocks, block_rows;
-  int per, wanted, n_ranges, n_wide, max_chunks;
+  int per, wanted, n_ranges, wide_rows, n_wide, max_chunks;
 };
 // Every range costs a compute unit about the bytes of its rows and of its adapter's weights, and ends with its adapter: `per` is the smallest size from
 // this one on that makes no more ranges than a multiple of the units (264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 take 20: 8192 rows of 8 KB).
-// `least`: rows that share the weights at least.
-static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int least) {
+// `least`: rows that share the weights at least.  `wide_rows`: rows of a range of `expand`, 16, 32 or 64.
+static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int least, int wide_rows) {
   p->rows = (int)rows; p->n_adapters = n_adapters;
   p->block_rows = rows <= LR_CUS * 1024 ? 1024 : (int)align_up((size_t)ceil_div(rows, LR_CUS), 1024);
   p->blocks = (int)ceil_div(rows > 0 ? rows : 1, p->block_rows);
@@ -35,7 +35,8 @@ static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int 
   if (p->per < least) p->per = least;
   const int64_t most = rows / LR_RANGE + n_adapters + 1;
   p->n_ranges = (int)(p->wanted > most ? p->wanted : most);
-  p->n_wide = (int)(rows / LR_WIDE + n_adapters + 1);
+  p->wide_rows = wide_rows;
+  p->n_wide = (int)(rows / wide_rows + n_adapters + 1);
   p->max_chunks = (int)(rows / LR_CHUNK + n_adapters);
   char *at = (char *)mem;
   auto take = [&](size_t bytes) { char *r = at; at += align_up(bytes, 16); return r; };
@@ -80,6 +81,7 @@ struct Lowrank {
   Dropout drop;
   Plan plan;
   int rt, rp, es;
+  bool both;      // `shrink` and `expand` in one kernel
   int64_t ht_ld;
   // saved by the forward pass (beside the plan)
   float *ht;

@@ -158,11 +158,11 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
   if (t < G && me == 0) p.slots[t] = {at[2], chunks};
   __syncthreads();
   const unsigned per = (unsigned)s_per;
-  int rat[2] = {(int)((unsigned)(n + per - 1) / per), (n + LR_WIDE - 1) / LR_WIDE}, rsum[2];
+  int rat[2] = {(int)((unsigned)(n + per - 1) / per), (n + p.wide_rows - 1) / p.wide_rows}, rsum[2];
   block_scan(rat, rsum, s_w);
   if (t < G) { s.range0[t] = rat[0]; s.wide0[t] = rat[1]; }
   if (t == 0) {
-    s.wide0[G] = rsum[1]; s.wide0[G + 1] = rsum[1] + (idle + LR_WIDE - 1) / LR_WIDE;
+    s.wide0[G] = rsum[1]; s.wide0[G + 1] = rsum[1] + (idle + p.wide_rows - 1) / p.wide_rows;
     s.range0[G] = rsum[0]; s.range0[G + 1] = rsum[0] + (int)((unsigned)(idle + per - 1) / per);
   }
   // where each wave's rows of each group go: 16 lanes a group
@@ -257,8 +257,12 @@ static void lowrank_layout(Lowrank *q, const gsdf_lowrank_args *a, void *save, v
   q->es = a->dtype == GSDF_F32 ? 4 : 2;
   q->ht_ld = (int64_t)align_up((size_t)a->rows + 32, 4);      // `outer` reads whole steps of 32 places
   Plan unused;
+  q->both = a->rows >= LR_BOTH && q->rt <= 2 && a->rank % 4 == 0;
+  // 64 rows of `expand` read the weights once; fewer rows where there are not enough waves otherwise
+  const int64_t chunks = ceil_div(a->n_in > a->n_out ? a->n_in : a->n_out, 64);
+  const int wide = q->both || a->rows / 64 * chunks < 2048 ? (!q->both && a->rows / 32 * chunks < 2048 ? 16 : 32) : 64;
   const int least = 4 * q->rt;      // (an adapter's weights are read once a range: the wider, the more rows have to share them)
-  const size_t plan_bytes = plan_layout(&unused, nullptr, a->rows, a->n_adapters, least), h_bytes = (size_t)a->rows * q->rp * 4, ht_bytes = (size_t)q->ht_ld * q->rp * 4;
+  const size_t plan_bytes = plan_layout(&unused, nullptr, a->rows, a->n_adapters, least, wide), h_bytes = (size_t)a->rows * q->rp * 4, ht_bytes = (size_t)q->ht_ld * q->rp * 4;
   Carve s(save), f(ws), b(ws);
   void *plan_saved = s.take<char>(plan_bytes);
   q->ht = s.take<float>(ht_bytes);
@@ -271,7 +275,7 @@ static void lowrank_layout(Lowrank *q, const gsdf_lowrank_args *a, void *save, v
   q->h = f.take<float>(h_bytes);
   q->a_frag = f.take<char>(weights * align_up((size_t)a->n_in, step));
   q->fwd_ws_bytes = f.used;      // the plan at least: never 0
-  plan_layout(&q->plan, training ? plan_saved : plan_ws, a->rows, a->n_adapters, least);
+  plan_layout(&q->plan, training ? plan_saved : plan_ws, a->rows, a->n_adapters, least, wide);
   q->dh = b.take<float>(h_bytes);
   q->dht = b.take<float>(ht_bytes);
   q->part[0] = b.take<float>(part * a->n_in);

@@ -150,7 +150,7 @@ __device__ __forceinline__ float scale_to_one(float largest) {
 
 // ---- shrink: H[place][j] = factor sum_k drop(x)[row][k] W[g][j][k] -------------------------------------------------------------------------
 // A workgroup of `split` waves has a range of rows and its waves take the steps of 128 bytes in turn (one wave: four ranges a workgroup).
-// RT: tiles of 16 ranks.  H: [places][16 RT] (for `expand`) and / or HT: [16 RT][ht_ld] (for `outer`), zeros behind the rank.
+// RT: tiles of 16 ranks.  H: [places][16 RT] (for `expand`; zeros behind the rank) and / or HT: [rank][ht_ld] (for `outer`).
 struct ShrinkArgs {
   const void *x, *w;
   int64_t x_stride;               // elements between rows
@@ -163,12 +163,10 @@ struct ShrinkArgs {
   Plan plan;
 };
 template <typename T, int RT, int TT, bool DROP, bool RAGGED>      // TT: tiles of 16 rows in the range
-__device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, int which, int part, f32x4 *s_sum) {
-  constexpr int RR = RT < 2 ? RT : 2;      // tiles of ranks that meet in LDS at a time
+__device__ __forceinline__ void shrink_sums(const ShrinkArgs &q, int4 range, int which, int part, f32x4 (&acc)[RT][TT]) {
   typedef typename Vec<T>::vec V;
   constexpr int N = Vec<T>::N, STEP = 8 * N;
   const int lane = threadIdx.x & 63, c = lane & 15, quad = lane >> 4;
-  f32x4 acc[RT][TT];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -210,22 +208,21 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[r][t] = mma(ws[r][i], xs[t][i], acc[r][t]);
   };
-  constexpr int AHEAD = RT == 1 && TT < 3 ? 4 : RT <= 4 ? 2 : 1;      // steps whose loads are on their way together
   int s = part;
-  for (; s + (AHEAD - 1) * q.split < full; s += AHEAD * q.split) {
-    V xs[AHEAD][TT][2], ws[AHEAD][RT][2];
+  auto steps = [&](auto ahead) {      // steps whose loads are on their way together
+    constexpr int AHEAD = decltype(ahead)::value;
+    for (; s + (AHEAD - 1) * q.split < full; s += AHEAD * q.split) {
+      V xs[AHEAD][TT][2], ws[AHEAD][RT][2];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) load(place(s + u * q.split), xs[u], ws[u]);
-    __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler saves registers and lets two loads go at a time)
+      for (int u = 0; u < AHEAD; ++u) load(place(s + u * q.split), xs[u], ws[u]);
+      __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler saves registers and lets two loads go at a time)
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) add(place(s + u * q.split), xs[u], ws[u]);
-  }
-  for (; s < full; s += q.split) {
-    V xs[TT][2], ws[RT][2];
-    load(place(s), xs, ws);
-    __builtin_amdgcn_sched_barrier(0);
-    add(place(s), xs, ws);
-  }
+      for (int u = 0; u < AHEAD; ++u) add(place(s + u * q.split), xs[u], ws[u]);
+    }
+  };
+  if (RT == 1 && TT < 3) steps(std::integral_constant<int, 4>{});
+  if (RT <= 4) steps(std::integral_constant<int, 2>{});
+  steps(std::integral_constant<int, 1>{});
   if (RAGGED && part == full % q.split) {      // the rows' last elements
     const int k = full * STEP + quad * N;
     V xs[TT][2], ws[RT][2];
@@ -238,6 +235,13 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
     }
     add(full, xs, ws);
   }
+}
+template <typename T, int RT, int TT, bool DROP, bool RAGGED>
+__device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, int which, int part, f32x4 *s_sum) {
+  constexpr int RR = RT < 2 ? RT : 2;      // tiles of ranks that meet in LDS at a time
+  const int lane = threadIdx.x & 63, c = lane & 15, quad = lane >> 4;
+  f32x4 acc[RT][TT];
+  shrink_sums<T, RT, TT, DROP, RAGGED>(q, range, which, part, acc);
   const float f = q.factor * (q.scales != nullptr ? q.scales[range.x] : 1.f);
   auto put = [&](int r, int t, f32x4 v) {
     const int i0 = t * 16 + c, j0 = r * 16 + quad * 4;
@@ -247,7 +251,8 @@ __device__ __forceinline__ void shrink_range(const ShrinkArgs &q, int4 range, in
     if (q.h != nullptr) *reinterpret_cast<f32x4 *>(q.h + (int64_t)(range.y + i0) * (16 * RT) + j0) = v;
     if (q.ht != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q.ht[(int64_t)(j0 + i) * q.ht_ld + range.y + i0] = v[i];
+      for (int i = 0; i < 4; ++i)
+        if (j0 + i < q.rank) q.ht[(int64_t)(j0 + i) * q.ht_ld + range.y + i0] = v[i];
     }
   };
   if (q.split == 1) {
@@ -312,8 +317,10 @@ __device__ __forceinline__ void change_halves(V &a_, V &b_, bool upper) {
   a_ = __builtin_bit_cast(V, a);
   b_ = __builtin_bit_cast(V, b);
 }
-template <typename T, int RT, int TT, bool DROP, bool RAGGED, bool PAST>
-__device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int part, int turn, int chunks) {
+// HERE: h comes from the wave's own sums, whose layout (a lane has 4 ranks of its row) an instruction takes as it is when the ranks of the contraction
+// are told the weights in that order: four high and four low parts a lane at 16 bits.  Else it is read from H.  `source` fills f.
+template <typename T, int RT, int TT, bool DROP, bool RAGGED, bool PAST, bool HERE, typename Source>
+__device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int part, int turn, int chunks, Source source) {
   typedef typename Vec<T>::vec V;
   constexpr int N = Vec<T>::N, NP = 8 / N;      // pairs of pieces of a lane's 16 columns: piece p at column 4 N p + N quad of the 64
   constexpr bool WIDE = sizeof(T) == 4;
@@ -366,26 +373,49 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
   const T *w = (const T *)q.w + range.x * q.w_group;
   // h of the lane's row as the instruction wants it.  16 bits: 8 ranks a lane, 32 an instruction, high and low parts (a rank of at most 16: both in
   // one instruction).  32 bits: 4 ranks a lane, 16 a group of four instructions.
-  constexpr int KB = WIDE ? RT : (RT == 1 ? 1 : RT / 2);
+  constexpr bool BOTH = !WIDE && (HERE || RT == 1);      // high and low parts in one instruction
+  constexpr int KB = WIDE || HERE ? RT : (RT == 1 ? 1 : RT / 2), FN = WIDE || HERE ? 1 : 2;
+  auto rank_of = [&](int k) { return WIDE || HERE ? k * 16 + quad * 4 : (RT == 1 ? (quad & 1) * 8 : k * 32 + quad * 8); };
+  V b[2 * TT][NP], u[4][KB];
+  auto load_weights = [&](int ch) {
+    const bool whole = !RAGGED || (ch * 64 + 64 <= q.width && (HERE || q.rank % N == 0));
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int col = ch * 64 + m * 4 / N * 4 * N + (c >> 2) * N + m * 4 % N + (c & 3);      // the column that this lane's weights belong to
+      const T *pw = w + (int64_t)(whole || col < q.width ? col : q.width - 1) * q.w_ld;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const int j = rank_of(k);
+        if constexpr (HERE && !WIDE) {      // (a rank that is a multiple of 4)
+          const typename Piece<T, 4>::vec four = *reinterpret_cast<const typename Piece<T, 4>::any *>(pw + (j < q.rank ? j : 0));
+          u[m][k] = V{four[0], four[1], four[2], four[3], four[0], four[1], four[2], four[3]};
+        } else if (whole || HERE) {
+          u[m][k] = load_vec<T>(pw + (j < q.rank ? j : 0));
+        } else {
+          u[m][k] = load_vec_end<T>(pw, j, q.rank);
+        }
+      }
+    }
+  };
+  auto chunk_of = [&](int i) { return i + turn < chunks ? i + turn : i + turn - chunks; };
+  load_weights(chunk_of(part));
+  load_base(chunk_of(part), b);
   V hi[TT][KB], lo[TT][KB];
   float back[TT];
   uint32_t row_of[TT];
-  auto rank_of = [&](int k) { return WIDE ? k * 16 + quad * 4 : (RT == 1 ? (quad & 1) * 8 : k * 32 + quad * 8); };
+  f32x4 f[TT][KB][FN];
+  source(f);
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int at = t * 16 + c < range.z ? t * 16 + c : range.z - 1;
-    if (DROP) row_of[t] = (uint32_t)order[at];
-    const float *ph = q.h + (int64_t)(range.y + at) * (16 * RT);
-    f32x4 f[KB][N / 4];
+    if (DROP) row_of[t] = (uint32_t)order[t * 16 + c < range.z ? t * 16 + c : range.z - 1];
     float largest = 0.f;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < N / 4; ++e) {
-        f[k][e] = *reinterpret_cast<const f32x4 *>(ph + rank_of(k) + e * 4);
-        if (DROP) f[k][e] *= q.drop.scale;
+      for (int e = 0; e < FN; ++e) {
+        if (DROP) f[t][k][e] *= q.drop.scale;
 #pragma unroll
-        for (int l = 0; l < 4; ++l) largest = fmaxf(largest, fabsf(f[k][e][l]));
+        for (int l = 0; l < 4; ++l) largest = fmaxf(largest, fabsf(f[t][k][e][l]));
       }
     float down = 1.f;
     back[t] = 1.f;
@@ -398,30 +428,21 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float v = f[k][e / 4][e % 4] * down;
+      for (int e = 0; e < FN * 4; ++e) {
+        const float v = f[t][k][e / 4][e % 4] * down;
         const T h = (T)v;
         const T l = (T)(v - (float)h);
-        hi[t][k][e] = !WIDE && RT == 1 && quad >= 2 ? l : h;
-        lo[t][k][e] = l;
+        if constexpr (HERE && !WIDE) {
+          hi[t][k][e] = h;
+          hi[t][k][e + 4] = l;
+        } else {
+          hi[t][k][e] = BOTH && quad >= 2 ? l : h;
+          lo[t][k][e] = l;
+        }
       }
   }
   for (int i = part; i < chunks; i += q.parts) {
-    const int ch = i + turn < chunks ? i + turn : i + turn - chunks;
-    const bool whole = !RAGGED || (ch * 64 + 64 <= q.width && q.rank % N == 0);
-    V b[2 * TT][NP], u[4][KB];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int col = ch * 64 + m * 4 / N * 4 * N + (c >> 2) * N + m * 4 % N + (c & 3);      // the column that this lane's weights belong to
-      const T *pw = w + (int64_t)(whole || col < q.width ? col : q.width - 1) * q.w_ld;
-#pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        const int j = rank_of(k);
-        if (whole) u[m][k] = load_vec<T>(pw + (j < q.rank ? j : 0));
-        else u[m][k] = load_vec_end<T>(pw, j, q.rank);
-      }
-    }
-    load_base(ch, b);
+    const int ch = chunk_of(i);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < 4; ++m)
@@ -436,7 +457,7 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
           acc[m] = mma(u[m][k], hi[t][k], acc[m]);
-          if (!WIDE && RT > 1) acc[m] = mma(u[m][k], lo[t][k], acc[m]);
+          if (!WIDE && !BOTH) acc[m] = mma(u[m][k], lo[t][k], acc[m]);
         }
       }
 #pragma unroll
@@ -467,8 +488,31 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
         store(2 * t + 1, ch * 64 + p * 8 * N + column, o[1]);
       }
     }
+    if (i + q.parts < chunks) {
+      load_weights(chunk_of(i + q.parts));
+      load_base(chunk_of(i + q.parts), b);
+    }
   }
 }
+// `source` of a range whose h is in memory: pieces of the lane's ranks
+template <typename T, int RT, int TT>
+struct FromMemory {
+  static constexpr bool WIDE = sizeof(T) == 4;
+  static constexpr int KB = WIDE ? RT : (RT == 1 ? 1 : RT / 2), FN = WIDE ? 1 : 2;
+  const float *h;      // of the range
+  int rows;
+  __device__ __forceinline__ void operator()(f32x4 (&f)[TT][KB][FN]) const {
+    const int c = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const float *p = h + (int64_t)(t * 16 + c < rows ? t * 16 + c : rows - 1) * (16 * RT) + (WIDE ? quad * 4 : RT == 1 ? (quad & 1) * 8 : quad * 8);
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int e = 0; e < FN; ++e) f[t][k][e] = *reinterpret_cast<const f32x4 *>(p + k * (16 * FN) + e * 4);
+    }
+  }
+};
 // RAGGED: the width is no multiple of 64 or the rank none of a lane's piece; PAST: y goes past the caches
 template <typename T, int RT, bool DROP, bool RAGGED, bool PAST>
 __global__ void __launch_bounds__(256, RAGGED || RT == 8 ? 1 : 2) lowrank_expand_kernel(ExpandArgs q) {
@@ -479,9 +523,46 @@ __global__ void __launch_bounds__(256, RAGGED || RT == 8 ? 1 : 2) lowrank_expand
   const int chunks = (q.width + 63) / 64, part = (int)(id % (unsigned)q.parts);
   const int turn = (int)(which % (unsigned)chunks);      // ranges begin at different columns: not all at the same memory channels
   if (DROP) dropout_counter(q.drop);
-  if (range.z > 32) expand_range<T, RT, 4, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
-  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
-  else expand_range<T, RT, 1, DROP, RAGGED, PAST>(q, range, part, turn, chunks);
+  const float *h = q.h + (int64_t)range.y * (16 * RT);
+  if (range.z > 32) expand_range<T, RT, 4, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 4>{h, range.z});
+  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 2>{h, range.z});
+  else expand_range<T, RT, 1, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 1>{h, range.z});
+}
+
+// ---- both: many rows leave no unit idle when a wave takes a range through `shrink` and `expand` by itself; h stays in its registers -------------
+template <typename T, int RT, int TT, bool DROP_X, bool DROP_Y, bool RAGGED, bool PAST>
+__device__ __forceinline__ void both_range(const ShrinkArgs &s, const ExpandArgs &q, int4 range, int which) {
+  const int c = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
+  auto source = [&](f32x4 (&f)[TT][RT][1]) {
+    f32x4 acc[RT][TT];
+    shrink_sums<T, RT, TT, DROP_X, RAGGED>(s, range, which, 0, acc);
+    const float factor = s.factor * (s.scales != nullptr ? s.scales[range.x] : 1.f);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int i0 = t * 16 + c, j0 = r * 16 + quad * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[t][r][0][i] = j0 + i < s.rank ? acc[r][t][i] * factor : 0.f;
+        if (s.ht != nullptr && i0 < range.z) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j0 + i < s.rank) s.ht[(int64_t)(j0 + i) * s.ht_ld + range.y + i0] = f[t][r][0][i];
+        }
+      }
+  };
+  expand_range<T, RT, TT, DROP_Y, RAGGED, PAST, true>(q, range, 0, which % ((q.width + 63) / 64), (q.width + 63) / 64, source);
+}
+template <typename T, int RT, bool DROP_X, bool DROP_Y, bool RAGGED, bool PAST>
+__global__ void __launch_bounds__(256) lowrank_both_kernel(ShrinkArgs s, ExpandArgs q) {
+  const int which = (int)__builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (which >= q.plan.n_wide) return;
+  const int4 range = q.plan.wide[which];
+  if (range.z == 0 || (range.x == q.plan.n_adapters && q.base == q.y)) return;
+  if (DROP_X) dropout_counter(s.drop);
+  if (DROP_Y) dropout_counter(q.drop);
+  if (range.z > 16) both_range<T, RT, 2, DROP_X, DROP_Y, RAGGED, PAST>(s, q, range, which);
+  else both_range<T, RT, 1, DROP_X, DROP_Y, RAGGED, PAST>(s, q, range, which);
 }
 
 // ---- outer: sum over an adapter's rows of UT[j][place] V[row][c] ----------------------------------------------------------------------------
@@ -541,9 +622,10 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
     for (int i = 0; i < 8; ++i) row[i] = order[at + i < chunk.z ? at + i : chunk.z - 1];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {      // (places behind the chunk are in the buffer, which has room behind its last)
-      const float *pu = s.ut + (int64_t)(rank0 + r * 16 + c) * q.ut_ld + chunk.y;
+      const int j = rank0 + r * 16 + c;
+      const float *pu = s.ut + (int64_t)(j < q.rank ? j : 0) * q.ut_ld + chunk.y;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) u[r][i] = load_vec<float>(pu + at + i * 4);
+      for (int i = 0; i < 2; ++i) u[r][i] = zero_unless<float>(rank0 + r * 16 + c < q.rank, load_vec<float>(pu + at + i * 4));
     }
     if (columns_whole) {
 #pragma unroll
@@ -761,43 +843,71 @@ static constexpr int64_t LR_PAST = 32 << 20;      // bytes of a result from whic
     default: { constexpr int RT = 8; __VA_ARGS__; break; }    \
   }
 
-template <typename T>
-static void shrink_launch(const Lowrank &q, const void *x, int64_t x_stride, int width, const void *w, const float *scales, bool drop, float *h, float *ht, hipStream_t stream) {
+static ShrinkArgs shrink_args(const Lowrank &q, const void *x, int64_t x_stride, int width, const void *w, const float *scales, bool drop, float *h, float *ht) {
   ShrinkArgs s;
-  s.x = x; s.w = w; s.x_stride = x_stride; s.width = width; s.rank = q.a.rank;
+  s.x = x; s.w = w; s.x_stride = x_stride; s.width = width; s.rank = q.a.rank; s.split = 1;
   s.scales = scales; s.factor = drop ? q.drop.scale : 1.f; s.h = h; s.ht = ht; s.ht_ld = q.ht_ld; s.drop = q.drop; s.plan = q.plan;
-  const int steps = (int)ceil_div(width, 128 / (int)sizeof(T));
-  s.split = steps >= 8 ? 8 : steps >= 4 ? 4 : steps >= 2 ? 2 : 1;
-  const unsigned grid = (unsigned)(s.split == 1 ? ceil_div(q.plan.n_ranges, 4) : q.plan.n_ranges), threads = s.split == 1 ? 256 : 64 * s.split;
-  const bool ragged = width % (128 / (int)sizeof(T)) != 0;
-  GSDF_BY_RANK(q.rt, {
-    const size_t lds = s.split == 1 ? 0 : (size_t)s.split * (RT < 2 ? 1 : 2) * 3 * 64 * sizeof(f32x4);
-    if (drop && ragged) lowrank_shrink_kernel<T, RT, true, true><<<grid, threads, lds, stream>>>(s);
-    else if (drop) lowrank_shrink_kernel<T, RT, true, false><<<grid, threads, lds, stream>>>(s);
-    else if (ragged) lowrank_shrink_kernel<T, RT, false, true><<<grid, threads, lds, stream>>>(s);
-    else lowrank_shrink_kernel<T, RT, false, false><<<grid, threads, lds, stream>>>(s);
-  });
+  return s;
 }
-template <typename T>
-static void expand_launch(const Lowrank &q, const float *h, const void *w, int64_t w_group, int w_ld, int ranks, int width, const void *base,
-                          int64_t base_stride, void *y, int64_t y_stride, bool drop, hipStream_t stream) {
+static ExpandArgs expand_args(const Lowrank &q, const float *h, const void *w, int64_t w_group, int w_ld, int ranks, int width, const void *base, int64_t base_stride,
+                              void *y, int64_t y_stride) {
   ExpandArgs s;
   s.h = h; s.w = w; s.base = base; s.y = y; s.w_group = w_group; s.base_stride = base_stride; s.y_stride = y_stride; s.width = width; s.w_ld = w_ld; s.rank = ranks;
-  s.drop = q.drop; s.plan = q.plan;
-  const int64_t chunks = ceil_div(width, 64);
+  s.parts = 1; s.drop = q.drop; s.plan = q.plan;
+  return s;
+}
+// y from x: `shrink` and `expand`, or both at once
+template <typename T>
+static void products_launch(const Lowrank &q, ShrinkArgs s, ExpandArgs e, bool drop_x, bool drop_y, hipStream_t stream) {
+  constexpr int STEP = 128 / (int)sizeof(T), N = 16 / (int)sizeof(T);
+  const bool past = (int64_t)q.a.rows * e.width * (int64_t)sizeof(T) >= LR_PAST;
+  if (q.both) {
+    const unsigned grid = (unsigned)ceil_div(q.plan.n_wide, 4);
+    const bool ragged = s.width % STEP != 0 || e.width % 64 != 0;
+    auto run = [&](auto rt, auto dx, auto dy) {
+      constexpr int RT = decltype(rt)::value;
+      constexpr bool DX = decltype(dx)::value, DY = decltype(dy)::value;
+      if (ragged) lowrank_both_kernel<T, RT, DX, DY, true, false><<<grid, 256, 0, stream>>>(s, e);
+      else if (past) lowrank_both_kernel<T, RT, DX, DY, false, true><<<grid, 256, 0, stream>>>(s, e);
+      else lowrank_both_kernel<T, RT, DX, DY, false, false><<<grid, 256, 0, stream>>>(s, e);
+    };
+    auto by_drop = [&](auto rt) {
+      if (drop_x) run(rt, std::true_type{}, std::false_type{});
+      else if (drop_y) run(rt, std::false_type{}, std::true_type{});
+      else run(rt, std::false_type{}, std::false_type{});
+    };
+    if (q.rt == 1) by_drop(std::integral_constant<int, 1>{});
+    else by_drop(std::integral_constant<int, 2>{});
+    return;
+  }
+  {
+    const int steps = (int)ceil_div(s.width, STEP);
+    s.split = steps >= 8 ? 8 : steps >= 4 ? 4 : steps >= 2 ? 2 : 1;
+    const unsigned grid = (unsigned)(s.split == 1 ? ceil_div(q.plan.n_ranges, 4) : q.plan.n_ranges), threads = s.split == 1 ? 256 : 64 * s.split;
+    const bool ragged = s.width % STEP != 0;
+    GSDF_BY_RANK(q.rt, {
+      const size_t lds = s.split == 1 ? 0 : (size_t)s.split * (RT < 2 ? 1 : 2) * 3 * 64 * sizeof(f32x4);
+      if (drop_x && ragged) lowrank_shrink_kernel<T, RT, true, true><<<grid, threads, lds, stream>>>(s);
+      else if (drop_x) lowrank_shrink_kernel<T, RT, true, false><<<grid, threads, lds, stream>>>(s);
+      else if (ragged) lowrank_shrink_kernel<T, RT, false, true><<<grid, threads, lds, stream>>>(s);
+      else lowrank_shrink_kernel<T, RT, false, false><<<grid, threads, lds, stream>>>(s);
+    });
+  }
+  if (e.y == nullptr) return;      // (dh alone is wanted)
+  const int64_t chunks = ceil_div(e.width, 64);
   // one chunk of 64 columns a wave until there are more than eight waves a SIMD, then more
-  s.parts = (int)ceil_div(chunks, ceil_div(chunks * q.plan.n_wide, LR_CUS * 4 * 8));
-  const unsigned grid = (unsigned)ceil_div((int64_t)q.plan.n_wide * s.parts, 4);
-  const bool ragged = width % 64 != 0 || ranks % (16 / (int)sizeof(T)) != 0, past = (int64_t)q.a.rows * width * (int64_t)sizeof(T) >= LR_PAST;
-  auto run = [&](auto rt, auto drop_) {
+  e.parts = (int)ceil_div(chunks, ceil_div(chunks * q.plan.n_wide, LR_CUS * 4 * 8));
+  const unsigned grid = (unsigned)ceil_div((int64_t)q.plan.n_wide * e.parts, 4);
+  const bool ragged = e.width % 64 != 0 || e.rank % N != 0;
+  auto run = [&](auto rt, auto drop) {
     constexpr int RT = decltype(rt)::value;
-    constexpr bool DROP = decltype(drop_)::value;
-    if (ragged) lowrank_expand_kernel<T, RT, DROP, true, false><<<grid, 256, 0, stream>>>(s);
-    else if (past) lowrank_expand_kernel<T, RT, DROP, false, true><<<grid, 256, 0, stream>>>(s);
-    else lowrank_expand_kernel<T, RT, DROP, false, false><<<grid, 256, 0, stream>>>(s);
+    constexpr bool DROP = decltype(drop)::value;
+    if (ragged) lowrank_expand_kernel<T, RT, DROP, true, false><<<grid, 256, 0, stream>>>(e);
+    else if (past) lowrank_expand_kernel<T, RT, DROP, false, true><<<grid, 256, 0, stream>>>(e);
+    else lowrank_expand_kernel<T, RT, DROP, false, false><<<grid, 256, 0, stream>>>(e);
   };
   GSDF_BY_RANK(q.rt, {
-    if (drop) run(std::integral_constant<int, RT>{}, std::true_type{});
+    if (drop_y) run(std::integral_constant<int, RT>{}, std::true_type{});
     else run(std::integral_constant<int, RT>{}, std::false_type{});
   });
 }
@@ -815,8 +925,8 @@ void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *
     return;
   }
   lowrank_plan_launch(q.plan, ids, lowrank_pack_args(q, training), stream);
-  shrink_launch<T>(q, a.x, a.x_stride, a.n_in, q.a_frag, a.scales, q.drop.threshold != 0, q.h, training ? q.ht : nullptr, stream);
-  expand_launch<T>(q, q.h, a.b, (int64_t)a.n_out * a.rank, a.rank, a.rank, a.n_out, base, base_stride, y, y_stride, false, stream);
+  products_launch<T>(q, shrink_args(q, a.x, a.x_stride, a.n_in, q.a_frag, a.scales, q.drop.threshold != 0, q.h, training ? q.ht : nullptr),
+                     expand_args(q, q.h, a.b, (int64_t)a.n_out * a.rank, a.rank, a.rank, a.n_out, base, base_stride, y, y_stride), q.drop.threshold != 0, false, stream);
 }
 
 template <typename T>
@@ -825,9 +935,8 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
   const bool drop = q.drop.threshold != 0;
   const unsigned G = (unsigned)a.n_adapters;
   if (a.rows > 0 && (dx != nullptr || da != nullptr))
-    shrink_launch<T>(q, dy, dy_stride, a.n_out, q.b_frag, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr, stream);
-  if (a.rows > 0 && dx != nullptr)
-    expand_launch<T>(q, q.dh, q.a_turned, (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride, drop, stream);
+    products_launch<T>(q, shrink_args(q, dy, dy_stride, a.n_out, q.b_frag, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr),
+                       expand_args(q, q.dh, q.a_turned, (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride), false, drop, stream);
   if (da == nullptr && db == nullptr) return;
   constexpr int COLS = 16 * (16 / (int)sizeof(T));
   OuterArgs o;
