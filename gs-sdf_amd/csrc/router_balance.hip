@@ -14,7 +14,7 @@
 
 namespace gsdf {
 
-static constexpr int RB_THREADS = 1024, RB_MAX_BLOCKS = 256, RB_MAX_EXPERTS = 1024;
+static constexpr int RB_THREADS = 1024, RB_MAX_BLOCKS = 256, RB_MAX_EXPERTS = GSDF_ROUTER_MAX_EXPERTS;
 
 // exp(x), x <= 0, in a few units in the last place: the product's rounding error goes back in (exp2's own is one unit)
 __device__ __forceinline__ float exp_fast(float x) {

@@ -735,6 +735,7 @@ int gsdf_lowrank_bwd(const gsdf_lowrank_args *args, const void *dy, int64_t dy_s
  *     loss = n_experts * sum_e (counts[e] / (k V)) (sum_valid p_te / V),       0 where V is 0.
  * fwd writes loss[1], counts[n_experts] and pull[n_experts] (for the backward pass); bwd writes v_logits [rows, n_experts] (contiguous) = v_loss[0] * dloss /
  * dlogits, 0 in rows that are not valid (whose logits may hold anything).  counts are constants of the gradient.  A row of -inf alone has p = 0. */
+#define GSDF_ROUTER_MAX_EXPERTS 1024
 size_t gsdf_router_balance_ws_bytes(int64_t rows, int n_experts);
 int gsdf_router_balance_fwd(int64_t rows, int n_experts, int k, int dtype, const void *logits, int64_t stride, const void *ids, int ids_64,
                             const uint8_t *mask, float *loss, int64_t *counts, float *pull, void *ws, gsdf_stream_t stream);

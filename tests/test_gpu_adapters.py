@@ -99,6 +99,15 @@ def test_lowrank_gradients_against_differences(ad):
         assert abs(got - slope) < 200 * 2.0 ** -24 * scale + 1e-9 * abs(at(0.0))
 
 
+def test_lowrank_without_base(ad):
+    x, a, b, ids, scales, _, dy = make(90, 40, 56, 8, 3, torch.float32, 0.1)
+    want = ref.Lowrank(x, a, b, ids, scales, None, dy)
+    x = x.view(30, 3, 40).requires_grad_(True)
+    y = ad.lowrank_adapt(x, a, b, ids.view(30, 3), scales)
+    want.check("y", y.view(90, 56), 48)
+    want.check("dx", torch.autograd.grad(y, x, dy.view(y.shape))[0].view(90, 40), 64)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows,k,n", [(5, 41, 23), (300, 41, 23), (300, 128, 64)])
 def test_lowrank_strided_rows_and_any_alignment(ad, dtype, rows, k, n):
