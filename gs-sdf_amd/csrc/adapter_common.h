@@ -23,12 +23,22 @@ __device__ __forceinline__ void load_piece(const T *__restrict__ p, T (&out)[N])
 #pragma unroll
   for (int i = 0; i < N; ++i) out[i] = t[i];
 }
-template <typename T, int N>
+template <typename T, int N, bool PAST = false>      // PAST: past the caches
 __device__ __forceinline__ void store_piece(T *__restrict__ p, const T (&in)[N]) {
   typename Piece<T, N>::vec t;
 #pragma unroll
   for (int i = 0; i < N; ++i) t[i] = in[i];
-  *reinterpret_cast<typename Piece<T, N>::any *>(p) = t;
+  if (PAST && N * sizeof(T) > 16) {      // (two accesses of 16 bytes)
+    typename Piece<T, N / 2>::vec a, b;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) { a[i] = t[i]; b[i] = t[N / 2 + i]; }
+    __builtin_nontemporal_store(a, reinterpret_cast<typename Piece<T, N / 2>::any *>(p));
+    __builtin_nontemporal_store(b, reinterpret_cast<typename Piece<T, N / 2>::any *>(p + N / 2));
+  } else if (PAST) {
+    __builtin_nontemporal_store(t, reinterpret_cast<typename Piece<T, N>::any *>(p));
+  } else {
+    *reinterpret_cast<typename Piece<T, N>::any *>(p) = t;
+  }
 }
 
 // ---- the dropout mask ---------------------------------------------------------------------------------------------------------------------

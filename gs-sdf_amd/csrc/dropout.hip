@@ -3,9 +3,13 @@
 // Streams x (and residual) once and writes y once: bound by memory at 32-bit elements; at 16-bit elements the generator's integer products
 // (20 per 8 elements, a quarter of the full rate) take about as long as the bytes.  One thread owns the 8 neighbouring elements of one Philox block,
 // 16 bits for each: the finest split that throws no random bits away.  Where x is dropped y is exactly 0 (or residual): an infinity or NaN there is gone.
+#include <type_traits>
+
 #include "adapter_common.h"
 
 namespace gsdf {
+
+static constexpr int64_t DROPOUT_PAST = 64 << 20;      // bytes of y from which on it is written past the caches
 
 // row = block index / blocks per row, by a multiplication: exact for numerators below 2^31
 struct FastDiv {
@@ -18,7 +22,8 @@ static FastDiv fast_div(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) { return (uint32_t)(((uint64_t)n * f.mul) >> 31 >> f.shift); }
 
-template <typename T, bool RESIDUAL>
+// PAST: y goes past the caches
+template <typename T, bool RESIDUAL, bool PAST>
 __global__ void __launch_bounds__(256)
     dropout_kernel(uint32_t n_blocks, FastDiv per_row, uint32_t row0, int64_t cols, const T *__restrict__ x, int64_t x_stride,
                    const T *__restrict__ residual, int64_t r_stride, Dropout d, T *__restrict__ y, int64_t y_stride) {
@@ -40,7 +45,7 @@ __global__ void __launch_bounds__(256)
         const float keep = dropout_keeps(d, w, j) ? (float)v[j] * d.scale : 0.f;
         v[j] = (T)(RESIDUAL ? keep + (float)r[j] : keep);
       }
-      store_piece<T, 8>(py, v);
+      store_piece<T, 8, PAST>(py, v);
     } else {
       dropout_bits(d, block, (uint32_t)row, w);
 #pragma unroll
@@ -60,10 +65,15 @@ static void dropout_launch(int64_t rows, int64_t cols, const T *x, int64_t x_str
   for (int64_t row0 = 0; row0 < rows; row0 += most_rows) {      // one launch unless the matrix has 2^34 elements
     const uint32_t n = (uint32_t)((rows - row0 < most_rows ? rows - row0 : most_rows) * per_row);
     const unsigned grid = (unsigned)ceil_div(n, 256) < 8192u ? (unsigned)ceil_div(n, 256) : 8192u;
-    if (residual != nullptr)
-      dropout_kernel<T, true><<<grid, 256, 0, stream>>>(n, fast_div((uint32_t)per_row), (uint32_t)row0, cols, x, x_stride, residual, r_stride, d, y, y_stride);
-    else
-      dropout_kernel<T, false><<<grid, 256, 0, stream>>>(n, fast_div((uint32_t)per_row), (uint32_t)row0, cols, x, x_stride, residual, r_stride, d, y, y_stride);
+    auto run = [&](auto res, auto past) {
+      dropout_kernel<T, decltype(res)::value, decltype(past)::value><<<grid, 256, 0, stream>>>(n, fast_div((uint32_t)per_row), (uint32_t)row0, cols, x, x_stride, residual,
+                                                                                            r_stride, d, y, y_stride);
+    };
+    const bool past = rows * cols * (int64_t)sizeof(T) >= DROPOUT_PAST;
+    if (residual != nullptr && past) run(std::true_type{}, std::true_type{});
+    else if (residual != nullptr) run(std::true_type{}, std::false_type{});
+    else if (past) run(std::false_type{}, std::true_type{});
+    else run(std::false_type{}, std::false_type{});
   }
 }
 

@@ -8,6 +8,7 @@ static constexpr int LR_CUS = 256;          // compute units the ranges are deal
 static constexpr int LR_AIM = 40;           // rows of a range that are aimed at, at most
 static constexpr int LR_RANGE = 48;         // most rows of a range: three matrix tiles
 static constexpr int LR_BOTH = 65536;        // rows from which on a wave takes a range through both products
+static constexpr int LR_PLAN_ONE = 16384;    // rows up to which the plan is one launch
 static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
 
 // ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------

@@ -85,7 +85,7 @@ __device__ __forceinline__ void pack_block(const PackArgs &q, int block) {
 }
 
 // The plan takes two launches: each workgroup counts its share of the rows; then each adds up the counts of all (they are few), finds where its own rows
-// go and puts them there.  One workgroup alone took 13 us for 8192 rows.
+// go and puts them there.  Up to 16384 rows each workgroup counts all rows instead, in one launch.
 __global__ void __launch_bounds__(1024) lowrank_plan_count_kernel(Plan p, Ids ids, PackArgs pack) {
   extern __shared__ int s_hist[];      // [n_adapters + 1]
   if ((int)blockIdx.x >= p.blocks) {
@@ -105,8 +105,15 @@ struct PlanLds {      // of lowrank_plan_place_kernel: all [n_adapters + 2], nex
   __host__ __device__ static size_t bytes(int G) { return (size_t)(6 * (G + 2) + 16 * (G + 1)) * 4; }
   __device__ explicit PlanLds(int *s, int G) : first(s), mine(s + G + 2), range0(s + 2 * (G + 2)), wide0(s + 5 * (G + 2)), chunk0(s + 3 * (G + 2)), slot0(s + 4 * (G + 2)), next(s + 6 * (G + 2)) {}
 };
-__global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids ids) {
+// ONE: no counts came before; each workgroup looks through all rows (LDS counters of 16 lanes each, so that rows of one adapter do not queue)
+template <bool ONE>
+__global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids ids, PackArgs pack) {
   extern __shared__ int s_mem[];
+  if (ONE && (int)blockIdx.x >= p.blocks) {
+    if (pack.es == 4) pack_block<uint32_t>(pack, blockIdx.x - p.blocks);
+    else pack_block<unsigned short>(pack, blockIdx.x - p.blocks);
+    return;
+  }
   __shared__ int s_w[16][4], s_all[1024], s_mine[1024], s_per;
   const int G = p.n_adapters, G1 = G + 1, t = threadIdx.x, lane = t & 63, wave = t >> 6, me = blockIdx.x;
   PlanLds s(s_mem, G);
@@ -114,27 +121,47 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
   const int first_row = me * p.block_rows, last_row = first_row + p.block_rows < p.rows ? first_row + p.block_rows : p.rows, run = p.block_rows / 16;
   const int from = first_row + wave * run, to = from + run < last_row ? from + run : last_row;
   const int h0 = from + lane < to ? group_of(ids, from + lane) : 0;      // (most shares have one row a lane: read once)
-  for (int i = t; i < 16 * G1; i += 1024) s.next[i] = 0;
   if (t == 0) s_per = LR_RANGE;
+  if (ONE) {
+    int *before = s.next, *others = s.next + 16 * G1;
+    for (int i = t; i < 32 * G1; i += 1024) before[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = t; i < p.rows; i += 1024) {
+      const int h = group_of(ids, i);
+      atomicAdd((i < first_row ? before : others) + (t & 15) * G1 + h, 1);
+    }
+    __syncthreads();
+    for (int h = t >> 4; h < G; h += 64) {
+      int b = before[(t & 15) * G1 + h], a = b + others[(t & 15) * G1 + h];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) { b += __shfl_xor(b, o, 16); a += __shfl_xor(a, o, 16); }
+      if ((t & 15) == 0) { s_all[h] = a; s_mine[h] = b; }
+    }
+    __syncthreads();
+  }
+  for (int i = t; i < 16 * G1; i += 1024) s.next[i] = 0;
   // the adapters' rows in all shares and in the shares before this one
   int width = 1, slices = 1;
-  while (width < G) width <<= 1;
-  while (slices < p.blocks && slices * width < 1024) slices <<= 1;
+  if (!ONE) {
+    while (width < G) width <<= 1;
+    while (slices < p.blocks && slices * width < 1024) slices <<= 1;
+  }
   const int slice = t / width, g = t & (width - 1);
   int all = 0, mine = 0;
-  if (g < G && slice < slices) {
+  if (!ONE && g < G && slice < slices) {
 #pragma unroll 4
     for (int b = slice; b < p.blocks; b += slices) {
       const int c = p.hist[(int64_t)b * G + g];
       all += c; mine += b < me ? c : 0;
     }
   }
-  s_all[t] = all; s_mine[t] = mine;
+  if (!ONE) { s_all[t] = all; s_mine[t] = mine; }
   __syncthreads();
   if (from + lane < to) atomicAdd(&s.next[wave * G1 + h0], 1);
   for (int i = from + 64 + lane; i < to; i += 64) atomicAdd(&s.next[wave * G1 + group_of(ids, i)], 1);
   for (int h = slices >> 1; h > 0; h >>= 1) {
-    if (slice < h) { s_all[t] += s_all[t + h * width]; s_mine[t] += s_mine[t + h * width]; }
+    if (!ONE && slice < h) { s_all[t] += s_all[t + h * width]; s_mine[t] += s_mine[t + h * width]; }
     __syncthreads();
   }
   const int n = t < G ? s_all[t] : 0, chunks = (n + LR_CHUNK - 1) / LR_CHUNK;
@@ -177,7 +204,7 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     s.next[w * G1 + h] = s.first[h] + s.mine[h] + i - c;
   }
   __syncthreads();
-  const int step = gridDim.x * 1024, ranges = s.range0[G + 1], n_chunks = s.chunk0[G];
+  const int step = p.blocks * 1024, ranges = s.range0[G + 1], n_chunks = s.chunk0[G];
   auto put = [&](int i, const int *range0, int count, int4 *out) {      // the ranges of an adapter are of about one size
     int4 r = {0, 0, 0, 0};
     if (i < count) {
@@ -221,8 +248,13 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
 }
 
 void lowrank_plan_launch(const Plan &p, const Ids &ids, const PackArgs &pack, hipStream_t stream) {
+  const size_t lds = PlanLds::bytes(p.n_adapters);
+  if (p.rows <= LR_PLAN_ONE && p.n_adapters <= 256) {
+    lowrank_plan_place_kernel<true><<<(unsigned)(p.blocks + pack.n_blocks), 1024, lds + (size_t)16 * (p.n_adapters + 1) * 4, stream>>>(p, ids, pack);
+    return;
+  }
   lowrank_plan_count_kernel<<<(unsigned)(p.blocks + pack.n_blocks), 1024, (size_t)(p.n_adapters + 1) * 4, stream>>>(p, ids, pack);
-  lowrank_plan_place_kernel<<<p.blocks, 1024, PlanLds::bytes(p.n_adapters), stream>>>(p, ids);
+  lowrank_plan_place_kernel<false><<<p.blocks, 1024, lds, stream>>>(p, ids, pack);
 }
 
 // a buffer in pieces of 256 bytes

@@ -774,17 +774,24 @@ __global__ void __launch_bounds__(256) lowrank_sum_kernel(SumArgs q) {
   ((T *)s.out)[g * n + i] = (T)v;
 }
 
-// ---- a few rows without gradients: no order, a workgroup per row ----------------------------------------------------------------------------
+// ---- a few rows without gradients: no order, workgroups of a row ---------------------------------------------------------------------------
+struct RowArgs {
+  Ids ids;
+  const void *x, *a, *b, *base;
+  void *y;
+  float *h;
+  int64_t x_stride, base_stride, y_stride;
+  int n_in, n_out, rank;
+  const float *scales;
+  Dropout drop;
+};
+// h_j of the row, in lane 63 of the wave
 template <typename T>
-__global__ void __launch_bounds__(1024) lowrank_row_shrink_kernel(Ids ids, const T *__restrict__ x, int64_t x_stride, const T *__restrict__ a, int width, int rank,
-                                                                  const float *__restrict__ scales, Dropout drop, float *__restrict__ h) {
+__device__ __forceinline__ float row_rank(const RowArgs &q, const Dropout &drop, int64_t row, int g, int j) {
   typedef typename Vec<T>::vec V;
   constexpr int N = Vec<T>::N;
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63, j = blockIdx.y * 16 + (threadIdx.x >> 6), g = group_of(ids, row);
-  if (j >= rank || g == ids.n_adapters) return;
-  dropout_counter(drop);
-  const T *px = x + row * x_stride, *pa = a + ((int64_t)g * rank + j) * width;
+  const int lane = threadIdx.x & 63, width = q.n_in;
+  const T *px = (const T *)q.x + row * q.x_stride, *pa = (const T *)q.a + ((int64_t)g * q.rank + j) * width;
   float s = 0.f;
   auto add = [&](int k, V u, V v) {
     if (drop.threshold != 0) drop_vec(drop, (uint32_t)row, k, u);
@@ -801,38 +808,97 @@ __global__ void __launch_bounds__(1024) lowrank_row_shrink_kernel(Ids ids, const
   }
   for (; k + N <= width; k += 64 * N) add(k, load_vec<T>(px + k), load_vec<T>(pa + k));
   if (k < width) add(k, load_vec_end<T>(px, k, width), load_vec_end<T>(pa, k, width));
-  s = wave_sum_to_lane63(s);
-  if (lane == 63) h[row * rank + j] = s * (scales != nullptr ? scales[g] : 1.f) * (drop.threshold != 0 ? drop.scale : 1.f);
+  return wave_sum_to_lane63(s) * (q.scales != nullptr ? q.scales[g] : 1.f) * (drop.threshold != 0 ? drop.scale : 1.f);
 }
-// 64 columns a step, four lanes to a column
-template <typename T>
-__global__ void __launch_bounds__(256) lowrank_row_expand_kernel(Ids ids, const float *__restrict__ h, const T *__restrict__ b, int width, int rank, const T *base,
-                                                                 int64_t base_stride, T *y, int64_t y_stride) {
+// columns n, n + step, .. of the row: LPC lanes a column, a lane 16 bytes of its weights at a time; h in LDS or in memory
+template <typename T, int LPC>
+__device__ __forceinline__ void row_columns(const RowArgs &q, int64_t row, int g, int n, int step, const float *h) {
+  typedef typename Vec<T>::vec V;
   constexpr int N = Vec<T>::N;
-  const int64_t row = blockIdx.x;
-  const int g = group_of(ids, row), sub = threadIdx.x & 3;
-  if (g == ids.n_adapters && base == y) return;
-  const float *ph = h + row * rank;
-  for (int n = blockIdx.y * 64 + (threadIdx.x >> 2); n < width; n += gridDim.y * 64) {
-    const float add = base != nullptr ? (float)base[row * base_stride + n] : 0.f;
-    float s = 0.f;
-    if (g < ids.n_adapters) {
-      const T *pb = b + ((int64_t)g * width + n) * rank;
-      for (int j = sub * N; j < rank; j += 4 * N) {
-        const typename Vec<T>::vec v = j + N <= rank ? load_vec<T>(pb + j) : load_vec_end<T>(pb, j, rank);
+  const int sub = threadIdx.x % LPC, rank = q.rank;
+  const bool has = g < q.ids.n_adapters;
+  const T *base = (const T *)q.base + row * q.base_stride, *pb = (const T *)q.b + (int64_t)g * q.n_out * rank;
+  T *y = (T *)q.y + row * q.y_stride;
+  constexpr int C = 4;      // columns on their way together
+  for (; n < q.n_out; n += C * step) {
+    float v[C], s[C];
 #pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(j + i < rank ? ph[j + i] : 0.f, (float)v[i], s);
+    for (int c = 0; c < C; ++c) {
+      const int at = n + c * step;
+      v[c] = q.base != nullptr && at < q.n_out ? (float)base[at] : 0.f;
+      s[c] = 0.f;
+    }
+    if (has) {
+      for (int j = sub * N; j < rank; j += LPC * N) {
+        V w[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const T *p = pb + (int64_t)(n + c * step < q.n_out ? n + c * step : n) * rank;
+          w[c] = j + N <= rank ? load_vec<T>(p + j) : load_vec_end<T>(p, j, rank);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float t = j + i < rank ? h[j + i] : 0.f;
+#pragma unroll
+          for (int c = 0; c < C; ++c) s[c] = fmaf(t, (float)w[c][i], s[c]);
+        }
       }
     }
-    s += __shfl_xor(s, 1);
-    s += __shfl_xor(s, 2);
-    if (sub == 0) y[row * y_stride + n] = (T)(s + add);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int o = 1; o < LPC; o <<= 1) s[c] += __shfl_xor(s[c], o);
+      if (sub == 0 && n + c * step < q.n_out) y[n + c * step] = (T)(s[c] + v[c]);
+    }
   }
+}
+template <typename T>
+__device__ __forceinline__ void row_columns_by_rank(const RowArgs &q, int64_t row, int g, int block, int blocks, const float *h) {
+  constexpr int N = Vec<T>::N;
+  const int t = threadIdx.x, threads = blockDim.x;
+  if (q.rank <= N) row_columns<T, 1>(q, row, g, block * threads + t, blocks * threads, h);
+  else if (q.rank <= 2 * N) row_columns<T, 2>(q, row, g, (block * threads + t) / 2, blocks * threads / 2, h);
+  else row_columns<T, 4>(q, row, g, (block * threads + t) / 4, blocks * threads / 4, h);
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) lowrank_row_shrink_kernel(RowArgs q) {
+  const int64_t row = blockIdx.x;
+  const int j = blockIdx.y * 16 + (threadIdx.x >> 6), g = group_of(q.ids, row);
+  if (j >= q.rank || g == q.ids.n_adapters) return;
+  dropout_counter(q.drop);
+  const float v = row_rank<T>(q, q.drop, row, g, j);
+  if ((threadIdx.x & 63) == 63) q.h[row * q.rank + j] = v;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) lowrank_row_expand_kernel(RowArgs q) {
+  const int64_t row = blockIdx.x;
+  const int g = group_of(q.ids, row);
+  if (g == q.ids.n_adapters && q.base == q.y) return;
+  row_columns_by_rank<T>(q, row, g, blockIdx.y, gridDim.y, q.h + row * q.rank);
+}
+// both in one launch: every workgroup of a row makes its h again
+template <typename T>
+__global__ void __launch_bounds__(1024) lowrank_row_kernel(RowArgs q) {
+  __shared__ float s_h[GSDF_LOWRANK_MAX_RANK];
+  const int64_t row = blockIdx.x;
+  const int g = group_of(q.ids, row);
+  if (g == q.ids.n_adapters && q.base == q.y) return;
+  if (g < q.ids.n_adapters) {
+    dropout_counter(q.drop);
+    for (int j = threadIdx.x >> 6; j < q.rank; j += 16) {
+      const float v = row_rank<T>(q, q.drop, row, g, j);
+      if ((threadIdx.x & 63) == 63) s_h[j] = v;
+    }
+  }
+  __syncthreads();
+  row_columns_by_rank<T>(q, row, g, blockIdx.y, gridDim.y, s_h);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------------
 // without gradients: so few rows that an adapter's weights are hardly read twice take no plan
 static constexpr int64_t LR_FEW_ROWS = 64;
+// bytes of A that may be read to make every row's h again in each of its workgroups, for a launch less
+static constexpr int64_t LR_ROW_AGAIN = 4 << 20;
 static constexpr int64_t LR_PAST = 32 << 20;      // bytes of a result from which on it is written past the caches
 
 #define GSDF_BY_RANK(rt, ...)                                 \
@@ -917,11 +983,19 @@ void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *
   const gsdf_lowrank_args &a = q.a;
   const Ids ids = {a.ids, a.ids_64, a.n_adapters};
   if (!training && (a.rows <= LR_FEW_ROWS || a.rows <= 4 * (int64_t)a.n_adapters)) {
-    lowrank_row_shrink_kernel<T><<<dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, 16)), 1024, 0, stream>>>(ids, (const T *)a.x, a.x_stride, (const T *)a.a, a.n_in, a.rank,
-                                                                                                         a.scales, q.drop, q.h);
-    lowrank_row_expand_kernel<T><<<dim3((unsigned)a.rows, (unsigned)(ceil_div(a.n_out, 64) < 4096 ? ceil_div(a.n_out, 64) : 4096)), 256, 0, stream>>>(
-        ids, q.h, (const T *)a.b, a.n_out, a.rank, (const T *)base,
-                                                                                                         base_stride, (T *)y, y_stride);
+    constexpr int N = 16 / (int)sizeof(T);
+    RowArgs r;
+    r.ids = ids; r.x = a.x; r.a = a.a; r.b = a.b; r.base = base; r.y = y; r.h = q.h; r.x_stride = a.x_stride; r.base_stride = base_stride; r.y_stride = y_stride;
+    r.n_in = a.n_in; r.n_out = a.n_out; r.rank = a.rank; r.scales = a.scales; r.drop = q.drop;
+    const int lanes = a.rank <= N ? 1 : a.rank <= 2 * N ? 2 : 4;
+    const int64_t wide = ceil_div((int64_t)a.n_out * lanes, 1024), weights = (int64_t)a.rank * a.n_in * (int64_t)sizeof(T);
+    if (a.rows * wide * weights <= LR_ROW_AGAIN) {
+      lowrank_row_kernel<T><<<dim3((unsigned)a.rows, (unsigned)wide), 1024, 0, stream>>>(r);
+      return;
+    }
+    const int64_t narrow = ceil_div((int64_t)a.n_out * lanes, 256), most = ceil_div(2048, a.rows);
+    lowrank_row_shrink_kernel<T><<<dim3((unsigned)a.rows, (unsigned)ceil_div(a.rank, 16)), 1024, 0, stream>>>(r);
+    lowrank_row_expand_kernel<T><<<dim3((unsigned)a.rows, (unsigned)(narrow < most ? narrow : most)), 256, 0, stream>>>(r);
     return;
   }
   lowrank_plan_launch(q.plan, ids, lowrank_pack_args(q, training), stream);
