@@ -6,32 +6,35 @@
 
 namespace gsdf {
 
-// exclusive sums of C numbers over the 1024 threads of the workgroup; totals in `sum`
+// inclusive sums over the lanes of the wave, without LDS
+__device__ __forceinline__ int wave_scan(int v) {
+  v += (int)dpp_mov_u<0x111>((unsigned)v);                   // row_shr:1, 2, 4, 8: inside rows of 16 lanes
+  v += (int)dpp_mov_u<0x112>((unsigned)v);
+  v += (int)dpp_mov_u<0x114>((unsigned)v);
+  v += (int)dpp_mov_u<0x118>((unsigned)v);
+  v += (int)dpp_mov_u<0x142, 0xA, 0xF, false>((unsigned)v);  // row_bcast:15 into rows 1 and 3
+  v += (int)dpp_mov_u<0x143, 0xC, 0xF, false>((unsigned)v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+// exclusive sums of C numbers (at most 4) over the 1024 threads of the workgroup; totals in `sum`
 template <int C>
-__device__ __forceinline__ void block_scan(int (&v)[C], int (&sum)[C], int (*s_w)[4]) {
+__device__ __forceinline__ void block_scan(int (&v)[C], int (&sum)[C], int4 *s_w) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int i[C], before[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) { i[c] = v[c]; before[c] = sum[c] = 0; }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1)
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int u = __shfl_up(i[c], o);
-      i[c] += lane >= o ? u : 0;
-    }
-  if (lane == 63) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) s_w[wave][c] = i[c];
-  }
+  for (int c = 0; c < C; ++c) { i[c] = wave_scan(v[c]); before[c] = sum[c] = 0; }
+  if (lane == 63) s_w[wave] = int4{i[0], C > 1 ? i[C > 1 ? 1 : 0] : 0, C > 2 ? i[C > 2 ? 2 : 0] : 0, C > 3 ? i[C > 3 ? 3 : 0] : 0};
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 16; ++w)
+  for (int w = 0; w < 16; ++w) {
+    const int4 t = s_w[w];
+    const int part[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       before[c] = w == wave ? sum[c] : before[c];
-      sum[c] += s_w[w][c];
+      sum[c] += part[c];
     }
+  }
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < C; ++c) v[c] = before[c] + i[c] - v[c];
@@ -114,7 +117,8 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     else pack_block<unsigned short>(pack, blockIdx.x - p.blocks);
     return;
   }
-  __shared__ int s_w[16][4], s_all[1024], s_mine[1024], s_per;
+  __shared__ int4 s_w[16];
+  __shared__ int s_all[1024], s_mine[1024], s_per;
   const int G = p.n_adapters, G1 = G + 1, t = threadIdx.x, lane = t & 63, wave = t >> 6, me = blockIdx.x;
   PlanLds s(s_mem, G);
   // the share's rows: each wave owns a run of them, so that places follow the rows' order
@@ -172,9 +176,7 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
   for (int per = p.per + wave; per < LR_RANGE; per += 16) {
     int k = 0;
     for (int i = lane; i < G; i += 64) k += (int)((unsigned)(s_all[i] + per - 1) / (unsigned)per);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) k += __shfl_xor(k, o);
-    k += (int)((unsigned)(idle + per - 1) / (unsigned)per);
+    k = __builtin_amdgcn_readlane(wave_scan(k), 63) + (int)((unsigned)(idle + per - 1) / (unsigned)per);
     if (k <= p.wanted) {      // sizes behind it make no more
       if (lane == 0) atomicMin(&s_per, per);
       break;
@@ -182,7 +184,6 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
   }
   if (t < G) { s.first[t] = at[0]; s.chunk0[t] = at[1]; s.slot0[t] = at[2]; s.mine[t] = s_mine[t]; }
   if (t == 0) { s.first[G] = sum[0]; s.first[G + 1] = p.rows; s.chunk0[G] = sum[1]; s.mine[G] = first_row - sum[3]; }
-  if (t < G && me == 0) p.slots[t] = {at[2], chunks};
   __syncthreads();
   const unsigned per = (unsigned)s_per;
   int rat[2] = {(int)((unsigned)(n + per - 1) / per), (n + p.wide_rows - 1) / p.wide_rows}, rsum[2];
@@ -204,26 +205,29 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     s.next[w * G1 + h] = s.first[h] + s.mine[h] + i - c;
   }
   __syncthreads();
-  const int step = p.blocks * 1024, ranges = s.range0[G + 1], n_chunks = s.chunk0[G];
-  auto put = [&](int i, const int *range0, int count, int4 *out) {      // the ranges of an adapter are of about one size
-    int4 r = {0, 0, 0, 0};
-    if (i < count) {
-      const int h = find_group(range0, G1, i);
-      const unsigned k = i - range0[h], m = range0[h + 1] - range0[h], rows = s.first[h + 1] - s.first[h], size = rows / m, more = rows % m;
-      r = {h, s.first[h] + (int)(k * size + (k < more ? k : more)), (int)(size + (k < more ? 1u : 0u)), 0};
-    }
-    out[i] = r;
-  };
-  for (int i = me * 1024 + t; i < p.n_ranges; i += step) put(i, s.range0, ranges, p.range);
-  for (int i = me * 1024 + t; i < p.n_wide; i += step) put(i, s.wide0, s.wide0[G1], p.wide);
-  for (int i = me * 1024 + t; i < p.max_chunks; i += step) {
+  // (nothing is written to memory before the last barrier: a barrier waits for it)
+  if (t < G && me == 0) p.slots[t] = {at[2], chunks};
+  for (int i = me * 1024 + t; i < p.n_ranges + p.n_wide + p.max_chunks; i += p.blocks * 1024) {
+    const bool chunk = i >= p.n_ranges + p.n_wide, wide = !chunk && i >= p.n_ranges;
+    const int *of = chunk ? s.chunk0 : wide ? s.wide0 : s.range0;
+    const int at_list = i - (chunk ? p.n_ranges + p.n_wide : wide ? p.n_ranges : 0), count = of[chunk ? G : G1];
     int4 r = {0, 0, 0, -1};
-    if (i < n_chunks) {      // the chunks of an adapter are of one size, whole steps of 32 rows
-      const int h = find_group(s.chunk0, G, i), k = i - s.chunk0[h], m = s.chunk0[h + 1] - s.chunk0[h], rows = s.first[h + 1] - s.first[h];
-      const int size = ((rows + m - 1) / m + 31) / 32 * 32, a = k * size < rows ? k * size : rows, b = a + size < rows ? a + size : rows;
-      r = {h, s.first[h] + a, b - a, m > 1 ? s.slot0[h] + k : -1};
+    if (at_list < count) {
+      const int h = find_group(of, chunk ? G : G1, at_list);
+      const unsigned k = at_list - of[h], m = of[h + 1] - of[h], rows = s.first[h + 1] - s.first[h];
+      unsigned from, to;
+      if (chunk) {      // the chunks of an adapter are of one size, whole steps of 32 rows
+        const unsigned size = ((rows + m - 1) / m + 31) / 32 * 32;
+        from = k * size < rows ? k * size : rows;
+        to = from + size < rows ? from + size : rows;
+      } else {          // its ranges are of about one size
+        const unsigned size = rows / m, more = rows % m;
+        from = k * size + (k < more ? k : more);
+        to = from + size + (k < more ? 1u : 0u);
+      }
+      r = {h, s.first[h] + (int)from, (int)(to - from), chunk && m > 1 ? s.slot0[h] + (int)k : -1};
     }
-    p.chunk[i] = r;
+    (chunk ? p.chunk : wide ? p.wide : p.range)[at_list] = r;
   }
   int bits = 0;
   while ((1 << bits) < G1) ++bits;
