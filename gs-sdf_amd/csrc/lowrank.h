@@ -10,6 +10,7 @@ static constexpr int LR_RANGE = 48;         // most rows of a range: three matri
 static constexpr int LR_BOTH = 65536;        // rows from which on a wave takes a range through both products
 static constexpr int LR_PLAN_ONE = 16384;    // rows up to which the plan is one launch
 static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
+static constexpr int LR_CHUNK_FEW = 2048;   // the same where all rows are no more: then no adapter has two, and nothing is left to add up
 
 // ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------
 // All in one int32 buffer.  Group n_adapters holds the rows without an adapter.
@@ -17,11 +18,11 @@ struct Plan {
   int *order;      // [rows]: the row at each place, adapters one behind the other, rows of one adapter in their own order
   int4 *range;     // [n_ranges]: adapter, first place, rows (0: unused), -
   int4 *wide;      // [n_wide]: the same of up to wide_rows rows, for `expand`
-  int4 *chunk;     // [max_chunks]: adapter, first place, rows (0: unused), slot of its partial sums (-1: the adapter's only chunk)
+  int4 *chunk;     // [max_chunks]: adapter (-1: unused), first place, rows (0: an adapter without any), slot of its partial sums (-1: its only chunk)
   int2 *slots;     // [n_adapters]: first slot, chunks
   int *hist;       // [blocks][n_adapters]: rows of each adapter in each workgroup's share
   int rows, n_adapters, blocks, block_rows;
-  int per, wanted, n_ranges, wide_rows, n_wide, max_chunks;
+  int per, wanted, n_ranges, wide_rows, n_wide, chunk_rows, max_chunks;
 };
 // Every range costs a compute unit about the bytes of its rows and of its adapter's weights, and ends with its adapter: `per` is the smallest size from
 // this one on that makes no more ranges than a multiple of the units (264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 take 20: 8192 rows of 8 KB).
@@ -38,7 +39,8 @@ static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int 
   p->n_ranges = (int)(p->wanted > most ? p->wanted : most);
   p->wide_rows = wide_rows;
   p->n_wide = (int)(rows / wide_rows + n_adapters + 1);
-  p->max_chunks = (int)(rows / LR_CHUNK + n_adapters);
+  p->chunk_rows = rows <= LR_CHUNK_FEW ? LR_CHUNK_FEW : LR_CHUNK;
+  p->max_chunks = (int)(rows / p->chunk_rows + n_adapters);
   char *at = (char *)mem;
   auto take = [&](size_t bytes) { char *r = at; at += align_up(bytes, 16); return r; };
   p->range = (int4 *)take((size_t)p->n_ranges * 16);
@@ -52,7 +54,7 @@ static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int 
 // slots for the chunks of adapters with more than one: such an adapter has more than LR_CHUNK rows, so there are at most twice rows / LR_CHUNK of them
 static int64_t plan_max_slots(int64_t rows, int n_adapters) {
   const int64_t twice = 2 * (rows / LR_CHUNK) + 1, all = rows / LR_CHUNK + n_adapters;
-  return rows <= LR_CHUNK ? 0 : (twice < all ? twice : all);
+  return rows <= LR_CHUNK_FEW ? 0 : (twice < all ? twice : all);
 }
 
 struct Ids {

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     if (!ONE && slice < h) { s_all[t] += s_all[t + h * width]; s_mine[t] += s_mine[t + h * width]; }
     __syncthreads();
   }
-  const int n = t < G ? s_all[t] : 0, chunks = (n + LR_CHUNK - 1) / LR_CHUNK;
+  const int n = t < G ? s_all[t] : 0, chunks = t >= G ? 0 : n > p.chunk_rows ? (n + p.chunk_rows - 1) / p.chunk_rows : 1;
   int at[4] = {n, chunks, chunks > 1 ? chunks : 0, t < G ? s_mine[t] : 0}, sum[4];
   block_scan(at, sum, s_w);
   const int idle = p.rows - sum[0];
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(1024) lowrank_plan_place_kernel(Plan p, Ids id
     const bool chunk = i >= p.n_ranges + p.n_wide, wide = !chunk && i >= p.n_ranges;
     const int *of = chunk ? s.chunk0 : wide ? s.wide0 : s.range0;
     const int at_list = i - (chunk ? p.n_ranges + p.n_wide : wide ? p.n_ranges : 0), count = of[chunk ? G : G1];
-    int4 r = {0, 0, 0, -1};
+    int4 r = {chunk ? -1 : 0, 0, 0, -1};
     if (at_list < count) {
       const int h = find_group(of, chunk ? G : G1, at_list);
       const unsigned k = at_list - of[h], m = of[h + 1] - of[h], rows = s.first[h + 1] - s.first[h];
@@ -296,7 +296,7 @@ static void lowrank_layout(Lowrank *q, const gsdf_lowrank_args *a, void *save, v
   q->both = a->rows >= LR_BOTH && q->rt <= 2 && a->rank % 4 == 0;
   // 64 rows of `expand` read the weights once; fewer rows where there are not enough waves otherwise
   const int64_t chunks = ceil_div(a->n_in > a->n_out ? a->n_in : a->n_out, 64);
-  const int wide = q->both || a->rows / 64 * chunks < 2048 ? (!q->both && a->rows / 32 * chunks < 2048 ? 16 : 32) : 64;
+  const int wide = q->both || q->rt > 2 || a->rows / 64 * chunks < 2048 ? (!q->both && a->rows / 32 * chunks < 2048 ? 16 : 32) : 64;
   const int least = 4 * q->rt;      // (an adapter's weights are read once a range: the wider, the more rows have to share them)
   const size_t plan_bytes = plan_layout(&unused, nullptr, a->rows, a->n_adapters, least, wide), h_bytes = (size_t)a->rows * q->rp * 4, ht_bytes = (size_t)q->ht_ld * q->rp * 4;
   Carve s(save), f(ws), b(ws);

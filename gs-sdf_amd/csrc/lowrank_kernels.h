@@ -524,8 +524,13 @@ __global__ void __launch_bounds__(256, RAGGED || RT == 8 ? 1 : 2) lowrank_expand
   const int turn = (int)(which % (unsigned)chunks);      // ranges begin at different columns: not all at the same memory channels
   if (DROP) dropout_counter(q.drop);
   const float *h = q.h + (int64_t)range.y * (16 * RT);
-  if (range.z > 32) expand_range<T, RT, 4, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 4>{h, range.z});
-  else if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 2>{h, range.z});
+  if constexpr (RT <= 2) {      // (a wider rank's h would leave room for two waves a SIMD)
+    if (range.z > 32) {
+      expand_range<T, RT, 4, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 4>{h, range.z});
+      return;
+    }
+  }
+  if (range.z > 16) expand_range<T, RT, 2, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 2>{h, range.z});
   else expand_range<T, RT, 1, DROP, RAGGED, PAST, false>(q, range, part, turn, chunks, FromMemory<T, RT, 1>{h, range.z});
 }
 
@@ -598,7 +603,7 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
   const int block = blockIdx.x % q.blocks;
   const int4 chunk = q.plan.chunk[blockIdx.x / q.blocks];
-  if (chunk.z == 0) return;
+  if (chunk.x < 0) return;
   const bool second = block >= q.blocks0;
   const OuterSide &s = q.side[second];
   const int col0 = (block - (second ? q.blocks0 : 0)) * COLS, col = col0 + c * VE, valid = s.width - col;
@@ -742,7 +747,7 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
     }
   }
 }
-// the adapters that `outer` did not finish: the sum of several chunks, in their order, or zeros where there are no rows
+// the adapters that `outer` did not finish: the sum of several chunks, in their order
 struct SumArgs {
   OuterSide side[2];
   int rank, rank_padded, blocks0;
@@ -754,23 +759,21 @@ __global__ void __launch_bounds__(256) lowrank_sum_kernel(SumArgs q) {
   const OuterSide &s = q.side[second];
   const int g = blockIdx.y;
   const int2 slots = q.plan.slots[g];
-  if (slots.y == 1) return;
+  if (slots.y <= 1) return;
   const int64_t i = (int64_t)((int)blockIdx.x - (second ? q.blocks0 : 0)) * 256 + threadIdx.x, n = (int64_t)q.rank * s.width;
   if (i >= n) return;
+  const int64_t each = (int64_t)q.rank_padded * s.width;
+  const int64_t at = s.columns_first ? i / q.rank * q.rank_padded + i % q.rank : i;
+  const float *p = s.part + slots.x * each + at;
   float v = 0.f;
-  if (slots.y > 1) {
-    const int64_t each = (int64_t)q.rank_padded * s.width;
-    const int64_t at = s.columns_first ? i / q.rank * q.rank_padded + i % q.rank : i;
-    const float *p = s.part + slots.x * each + at;
-    int k = 0;
-    for (; k + 8 <= slots.y; k += 8) {
-      float t[8];
+  int k = 0;
+  for (; k + 8 <= slots.y; k += 8) {
+    float t[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = p[(k + i) * each];
-      v += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-    }
-    for (; k < slots.y; ++k) v += p[k * each];
+    for (int e = 0; e < 8; ++e) t[e] = p[(k + e) * each];
+    v += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   }
+  for (; k < slots.y; ++k) v += p[k * each];
   ((T *)s.out)[g * n + i] = (T)v;
 }
 
@@ -836,12 +839,22 @@ __device__ __forceinline__ void row_columns(const RowArgs &q, int64_t row, int g
           const T *p = pb + (int64_t)(n + c * step < q.n_out ? n + c * step : n) * rank;
           w[c] = j + N <= rank ? load_vec<T>(p + j) : load_vec_end<T>(p, j, rank);
         }
+        float t[N];
+        if (j + N <= rank) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float t = j + i < rank ? h[j + i] : 0.f;
+          for (int i = 0; i < N; i += 4) {
+            const Vec<float>::vec four = load_vec<float>(h + j + i);
 #pragma unroll
-          for (int c = 0; c < C; ++c) s[c] = fmaf(t, (float)w[c][i], s[c]);
+            for (int e = 0; e < 4; ++e) t[i + e] = four[e];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) t[i] = j + i < rank ? h[j + i] : 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int c = 0; c < C; ++c) s[c] = fmaf(t[i], (float)w[c][i], s[c]);
       }
     }
 #pragma unroll
@@ -1020,7 +1033,7 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
   o.blocks0 = da != nullptr ? (int)ceil_div(a.n_in, COLS) : 0;
   const unsigned blocks1 = db != nullptr ? (unsigned)ceil_div(a.n_out, COLS) : 0;
   o.blocks = o.blocks0 + (int)blocks1;
-  if (a.rows > 0) {
+  {
     const dim3 grid((unsigned)o.blocks * (unsigned)q.plan.max_chunks, q.rt == 8 ? 2 : 1);
     const bool ragged = a.n_in % COLS != 0 || a.n_out % COLS != 0;
     switch (q.rt) {
@@ -1029,6 +1042,7 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
       default: ragged ? lowrank_outer_kernel<T, 4, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 4, false><<<grid, 512, 0, stream>>>(o); break;
     }
   }
+  if (a.rows <= q.plan.chunk_rows) return;      // no adapter has two chunks
   SumArgs s;
   s.side[0] = o.side[0]; s.side[1] = o.side[1]; s.rank = a.rank; s.rank_padded = q.rp; s.plan = q.plan;
   s.blocks0 = da != nullptr ? (int)ceil_div((int64_t)a.rank * a.n_in, 256) : 0;
