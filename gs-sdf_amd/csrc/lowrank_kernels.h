@@ -142,6 +142,11 @@ __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 acc) {
   for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
   return acc;
 }
+// what rounding v to h left; an infinity leaves nothing
+template <typename T>
+__device__ __forceinline__ T low_part(float v, T h) {
+  return fabsf((float)h) == INFINITY ? (T)0.f : (T)(v - (float)h);
+}
 // a power of two that brings `largest` into [1, 2): 16-bit numbers of fp16 would run over or vanish
 __device__ __forceinline__ float scale_to_one(float largest) {
   const int e = (__float_as_int(largest) >> 23) & 255;
@@ -431,7 +436,7 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
       for (int e = 0; e < FN * 4; ++e) {
         const float v = f[t][k][e / 4][e % 4] * down;
         const T h = (T)v;
-        const T l = (T)(v - (float)h);
+        const T l = low_part<T>(v, h);
         if constexpr (HERE && !WIDE) {
           hi[t][k][e] = h;
           hi[t][k][e + 4] = l;
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
         for (int i = 0; i < 8; ++i) {
           const float t = u[r][i / 4][i % 4] * down;
           hi[r][i] = (T)t;
-          lo[r][i] = (T)(t - (float)hi[r][i]);
+          lo[r][i] = low_part<T>(t, hi[r][i]);
         }
       u32x4 words[8];
 #pragma unroll
@@ -908,7 +913,9 @@ __global__ void __launch_bounds__(1024) lowrank_row_kernel(RowArgs q) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------------
-// without gradients: so few rows that an adapter's weights are hardly read twice take no plan
+// Without gradients, few rows take no plan, which costs 10 us before the first product: where an adapter has hardly more than four of them, and where reading
+// the weights again for every row is no more than this (bf16, 4096 -> 4096: rank 16, 192 rows 12 us against 18, 64 rows of rank 128 16 to 24 against 33).
+static constexpr int64_t LR_FEW_BYTES = 32 << 20;
 static constexpr int64_t LR_FEW_ROWS = 64;
 // bytes of A that may be read to make every row's h again in each of its workgroups, for a launch less
 static constexpr int64_t LR_ROW_AGAIN = 4 << 20;
@@ -995,7 +1002,8 @@ template <typename T>
 void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *y, int64_t y_stride, bool training, hipStream_t stream) {
   const gsdf_lowrank_args &a = q.a;
   const Ids ids = {a.ids, a.ids_64, a.n_adapters};
-  if (!training && (a.rows <= LR_FEW_ROWS || a.rows <= 4 * (int64_t)a.n_adapters)) {
+  const int64_t read = a.rows * a.rank * ((int64_t)a.n_in + a.n_out) * (int64_t)sizeof(T);      // of the adapters' weights, row by row
+  if (!training && (a.rows <= LR_FEW_ROWS || a.rows <= 4 * (int64_t)a.n_adapters || (a.rows <= 8 * LR_FEW_ROWS && read <= LR_FEW_BYTES))) {
     constexpr int N = 16 / (int)sizeof(T);
     RowArgs r;
     r.ids = ids; r.x = a.x; r.a = a.a; r.b = a.b; r.base = base; r.y = y; r.h = q.h; r.x_stride = a.x_stride; r.base_stride = base_stride; r.y_stride = y_stride;

@@ -78,10 +78,10 @@ def test_balance_refuses(capi):
     f = lambda rows=4, e=8, k=1, dtype=0, logits=64, s=8, ids=64, loss=64, ws=64: L.gsdf_router_balance_fwd(  # noqa: E731
         rows, e, k, dtype, logits, s, ids, 0, None, loss, 64, 64, ws, None)
     for bad in (dict(rows=-1), dict(rows=1 << 31), dict(e=0), dict(e=1025), dict(k=0), dict(k=9), dict(dtype=-1), dict(logits=None), dict(ids=None), dict(loss=None),
-                dict(ws=None), dict(s=7)):
+                dict(ws=None), dict(s=-1)):
         assert f(**bad) == -1, bad
     b = lambda rows=4, e=8, dtype=0, logits=64, s=8, pull=64, v=64: L.gsdf_router_balance_bwd(rows, e, dtype, logits, s, None, pull, 64, v, None)  # noqa: E731
-    for bad in (dict(rows=-1), dict(e=0), dict(e=1025), dict(dtype=9), dict(logits=None), dict(pull=None), dict(v=None), dict(s=7)):
+    for bad in (dict(rows=-1), dict(e=0), dict(e=1025), dict(dtype=9), dict(logits=None), dict(pull=None), dict(v=None), dict(s=-1)):
         assert b(**bad) == -1, bad
     assert b(rows=0) == 0
 

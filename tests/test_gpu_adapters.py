@@ -36,7 +36,9 @@ SHAPES = [(1, 64, 64, 16, 1, 0.0, False), (1, 1, 1, 1, 1, 0.0, False), (2, 7, 5,
           (17, 129, 65, 17, 5, 0.0, False), (63, 200, 100, 64, 7, 0.2, True), (64, 256, 128, 32, 2, 0.0, True), (65, 72, 80, 128, 3, 0.0, False),
           (130, 1000, 1001, 12, 40, 0.1, False), (257, 40, 24, 100, 2, 0.5, False), (700, 136, 264, 16, 6, 0.05, False), (2500, 64, 64, 8, 6, 0.0, False),
           (5000, 32, 16, 4, 12, 0.1, True), (1500, 512, 96, 48, 9, 0.0, True), (3000, 16, 300, 20, 1000, 0.1, False), (900, 300, 16, 65, 1, 0.0, False),
-          (20000, 24, 40, 16, 9, 0.05, False), (40000, 8, 8, 2, 1024, 0.1, False), (70000, 64, 64, 8, 6, 0.05, False), (66000, 24, 72, 20, 5, 0.1, True), (65600, 72, 8, 4, 3, 0.0, False), (4500, 264, 136, 96, 3, 0.0, True)]
+          (20000, 24, 40, 16, 9, 0.05, False), (40000, 8, 8, 2, 1024, 0.1, False), (70000, 64, 64, 8, 6, 0.05, False), (66000, 24, 72, 20, 5, 0.1, True), (65600, 72, 8, 4, 3, 0.0, False),
+          (9500, 136, 72, 20, 3, 0.0, False), (9800, 72, 136, 64, 2, 0.0, True), (10000, 64, 64, 128, 3, 0.02, False), (8200, 1040, 1024, 16, 5, 0.0, False),
+          (8200, 64, 2112, 8, 5, 0.0, False), (48, 2048, 1024, 32, 4, 0.1, False), (2048, 64, 48, 8, 3, 0.0, False), (2049, 64, 48, 8, 1, 0.0, False), (4500, 264, 136, 96, 3, 0.0, True)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -264,6 +266,46 @@ def test_lowrank_rows_behind_32_bits(ad):
     assert torch.equal(d, ad.dropout(x, 0.3, 5))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,k,n,r", [(5, 200, 96, 16), (60, 2048, 1024, 32), (900, 136, 72, 12), (66000, 64, 64, 8)])
+def test_lowrank_one_mask_on_every_path(ad, rows, k, n, r, dtype):
+    """with and without gradients, few rows and many: the same elements are dropped"""
+    x, a, b, ids, scales, base, _ = make(rows, k, n, r, 4, dtype, 0.1)
+    want = ref.Lowrank(x, a, b, ids, scales, base, None, 0.3, 21, 22)
+    want.check("y", ad.lowrank_adapt(x, a, b, ids, scales, base, p=0.3, seed=21, offset=22), k + r)
+    want.check("y", ad.lowrank_adapt(x.requires_grad_(True), a, b, ids, scales, base, p=0.3, seed=21, offset=torch.tensor([22], device="cuda")), k + r)
+
+
+def test_lowrank_backward_twice_and_a_moved_counter(ad):
+    x, a, b, ids, scales, base, dy = make(300, 64, 48, 8, 3, torch.float32)
+    x.requires_grad_(True)
+    word = torch.tensor([5], device="cuda")
+    y = ad.lowrank_adapt(x, a, b, ids, scales, base, p=0.3, seed=1, offset=word)
+    z = ad.dropout(x, 0.3, 1, word)
+    first = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(y, x, dy, retain_graph=True)[0])
+    word += 1      # the masks of the forward passes are gone
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, dy)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z.sum(), x)
+
+
+def test_lowrank_infinite_factors(ad):
+    """32 bits: what the formula gives; 16 bits: not finite there, and nowhere else"""
+    for dtype in DTYPES:
+        for rows in (3, 200):
+            x, a, b, ids, scales, base, _ = make(rows, 40, 24, 1, 2, dtype)
+            a, b, x = a.abs() + 0.1, b.abs() + 0.1, x.abs() + 0.1
+            ids[:2] = torch.tensor([0, 1], device="cuda", dtype=torch.int32)
+            x[0, 7], b[1, 5] = math.inf, math.inf
+            y = ad.lowrank_adapt(x, a, b, ids, scales, base).float()
+            assert (y[0] == math.inf).all()
+            hit = torch.zeros_like(y, dtype=torch.bool)
+            hit[0], hit[ids == 1, 5] = True, True
+            assert torch.equal(~torch.isfinite(y), hit) and (dtype != torch.float32 or (y[hit] == math.inf).all())
+
+
 def test_lowrank_results_do_not_change_from_run_to_run(ad):
     x, a, b, ids, scales, base, dy = make(3000, 256, 192, 16, 7, torch.bfloat16, 0.1)
     leaves = [t.requires_grad_(True) for t in (x, a, b)]
@@ -385,6 +427,12 @@ def test_balance_edges(ad):
     wide = torch.full((40, 20), math.nan, device="cuda")
     wide[:, 3:15] = z.cuda()
     assert torch.equal(ad.router_balance(wide[:, 3:15], ids.cuda())[0], ad.router_balance(z.cuda(), ids.cuda())[0])
+    one = z[:1].expand(40, 12)
+    lg = z[:1].cuda().requires_grad_(True)
+    got = ad.router_balance(lg.expand(40, 12), ids.cuda())[0]
+    want = ref.Balance(one, ids)
+    assert abs(float(got.detach()) - float(want.loss)) <= float(want.loss_bound)
+    assert torch.allclose(torch.autograd.grad(got, lg)[0].cpu().double()[0], want.v.sum(dim=0), rtol=1e-4, atol=1e-7)
     lead = ad.router_balance(z.cuda().view(5, 8, 12), ids.cuda().view(5, 8, 2))
     assert torch.equal(lead[0], ad.router_balance(z.cuda(), ids.cuda())[0])
 
