@@ -942,12 +942,12 @@ static ExpandArgs expand_args(const Lowrank &q, const float *h, const void *w, i
   s.parts = 1; s.drop = q.drop; s.plan = q.plan;
   return s;
 }
-// y from x: `shrink` and `expand`, or both at once
+// y from x: `shrink` and `expand`, or both at once; `shrink` alone where no y is wanted
 template <typename T>
 static void products_launch(const Lowrank &q, ShrinkArgs s, ExpandArgs e, bool drop_x, bool drop_y, hipStream_t stream) {
   constexpr int STEP = 128 / (int)sizeof(T), N = 16 / (int)sizeof(T);
   const bool past = (int64_t)q.a.rows * e.width * (int64_t)sizeof(T) >= LR_PAST;
-  if (q.both) {
+  if (q.both && e.y != nullptr) {
     const unsigned grid = (unsigned)ceil_div(q.plan.n_wide, 4);
     const bool ragged = s.width % STEP != 0 || e.width % 64 != 0;
     auto run = [&](auto rt, auto dx, auto dy) {
@@ -979,7 +979,7 @@ static void products_launch(const Lowrank &q, ShrinkArgs s, ExpandArgs e, bool d
       else lowrank_shrink_kernel<T, RT, false, false><<<grid, threads, lds, stream>>>(s);
     });
   }
-  if (e.y == nullptr) return;      // (dh alone is wanted)
+  if (e.y == nullptr) return;      // dh alone: x wants no gradient
   const int64_t chunks = ceil_div(e.width, 64);
   // one chunk of 64 columns a wave until there are more than eight waves a SIMD, then more
   e.parts = (int)ceil_div(chunks, ceil_div(chunks * q.plan.n_wide, LR_CUS * 4 * 8));
@@ -1030,7 +1030,7 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
   const bool drop = q.drop.threshold != 0;
   const unsigned G = (unsigned)a.n_adapters;
   if (a.rows > 0 && (dx != nullptr || da != nullptr))
-    products_launch<T>(q, shrink_args(q, dy, dy_stride, a.n_out, q.b_frag, a.scales, false, q.dh, da != nullptr ? q.dht : nullptr),
+    products_launch<T>(q, shrink_args(q, dy, dy_stride, a.n_out, q.b_frag, a.scales, false, dx != nullptr ? q.dh : nullptr, da != nullptr ? q.dht : nullptr),
                        expand_args(q, q.dh, q.a_turned, (int64_t)a.n_in * q.rp, q.rp, q.rp, a.n_in, nullptr, 0, dx, dx_stride), false, drop, stream);
   if (da == nullptr && db == nullptr) return;
   constexpr int COLS = 16 * (16 / (int)sizeof(T));

@@ -85,6 +85,19 @@ def test_lowrank_one_gradient_at_a_time(ad, which):
     want.check("d" + which, torch.autograd.grad(y, leaf, dy)[0], 96 + 80 + 200)
 
 
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("rows,r", [(65536, 8), (66000, 24), (70001, 6), (9000, 64)])
+@pytest.mark.parametrize("which", ["x", "a", "b", "ab", "xb"])
+def test_lowrank_some_gradients_of_many_rows(ad, which, rows, r, p):
+    """the factors that want no gradient are left out on every path, the one that takes rows through both products at once among them"""
+    x, a, b, ids, scales, base, dy = make(rows, 40, 72, r, 5, torch.bfloat16, 0.1)
+    want = ref.Lowrank(x, a, b, ids, scales, base, dy, p, 5, 6)
+    leaves = [{"x": x, "a": a, "b": b}[w].requires_grad_(True) for w in which]
+    grads = torch.autograd.grad(ad.lowrank_adapt(x, a, b, ids, scales, base, p=p, seed=5, offset=6), leaves, dy)
+    for w, g in zip(which, grads):
+        want.check("d" + w, g, 40 + 72 + rows)
+
+
 def test_lowrank_gradients_against_differences(ad):
     """d/de of sum(y dy) along random directions, by differences of the 64-bit forward, against the kernels' gradients"""
     x, a, b, ids, scales, base, dy = make(90, 37, 29, 9, 5, torch.float32, 0.1)
