@@ -277,6 +277,8 @@ static int lowrank_check(const gsdf_lowrank_args *a) {
   GSDF_REQUIRE(a->n_in >= 1 && a->n_out >= 1 && a->n_in < (1 << 22) && a->n_out < (1 << 22), "lowrank: widths %d -> %d outside [1, 2^22)", a->n_in, a->n_out);
   GSDF_REQUIRE(a->rank >= 1 && a->rank <= GSDF_LOWRANK_MAX_RANK, "lowrank: rank %d outside [1, %d]", a->rank, GSDF_LOWRANK_MAX_RANK);
   GSDF_REQUIRE(a->n_adapters >= 1 && a->n_adapters <= GSDF_LOWRANK_MAX_ADAPTERS, "lowrank: %d adapters outside [1, %d]", a->n_adapters, GSDF_LOWRANK_MAX_ADAPTERS);
+  const int64_t weights = (int64_t)a->n_adapters * 16 * rank_tiles(a->rank) * (2 * (int64_t)a->n_in + a->n_out);
+  GSDF_REQUIRE(weights < (1ll << 32), "lowrank: %lld elements of weights (ranks in whole tiles of matrix instructions) are more than a launch can lay out", (long long)weights);
   GSDF_REQUIRE(known_dtype(a->dtype), "lowrank: unknown element type %d", a->dtype);
   GSDF_REQUIRE(a->p >= 0.0 && a->p <= 1.0, "lowrank: p = %g outside [0, 1]", a->p);
   GSDF_REQUIRE(a->rows == 0 || (a->x != nullptr && a->ids != nullptr), "lowrank: x and ids are required");

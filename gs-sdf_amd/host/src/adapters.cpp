@@ -172,6 +172,19 @@ LowrankCall lowrank_check(const Tensor &x, Tensor &a, Tensor &b, const Tensor &i
   return c;
 }
 
+// two matrices of one width of element in the same memory: apart, or columns of one buffer that do not meet
+void share_nothing(const Tensor &y, const Tensor &x) {
+  if (y.numel() == 0 || x.numel() == 0) return;
+  const int64_t rows = y.size(0), es = (int64_t)y.element_size(), n = y.size(1) * es, k = x.size(1) * es, stride = y.stride(0) * es;
+  const char *py = (const char *)y.data_ptr(), *px = (const char *)x.data_ptr();
+  if (py + (rows - 1) * stride + n <= px || px + (rows - 1) * x.stride(0) * es + k <= py) return;
+  if (rows > 1 && x.stride(0) == y.stride(0)) {
+    const int64_t by = ((px - py) % stride + stride) % stride;
+    if (by >= n && by + k <= stride) return;
+  }
+  TORCH_CHECK(false, "lowrank_adapt_: y and x share memory");
+}
+
 // ---- L2 -------------------------------------------------------------------------------------------------------------------------------------
 struct DropoutCall {
   Tensor word;
@@ -271,6 +284,7 @@ void lowrank_adapt_(const Tensor &y, const Tensor &x, const Tensor &a_, const Te
   TORCH_CHECK(out.stride(1) == 1 || out.size(1) == 1, "lowrank_adapt_: the elements of a row of y have to be neighbours");
   TORCH_CHECK(out.size(0) <= 1 || out.stride(0) >= out.size(1), "lowrank_adapt_: the rows of y overlap");
   const Tensor m = matrix(x);
+  share_nothing(out, m);
   lowrank_run(m, a, b, c, out, out, false);
   y.unsafeGetTensorImpl()->bump_version();
 }

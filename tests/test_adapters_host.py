@@ -53,6 +53,17 @@ def test_lowrank_refuses(capi, bad, said):
     assert said in L.gsdf_last_error().decode()
 
 
+def test_lowrank_refuses_weights_behind_a_launch(capi):
+    L = capi.lib()
+    for bad in (dict(n_adapters=1024, n_in=1 << 21, rank=1, x_stride=1 << 21), dict(n_adapters=1024, n_out=1 << 21, rank=4), dict(n_adapters=700, n_in=1 << 14, n_out=1 << 14, rank=65)):
+        args = _args(capi, **bad)
+        assert L.gsdf_lowrank_fwd(C.byref(args), None, 0, 64, 1 << 21, None, 64, None) == -1
+        assert "weights" in L.gsdf_last_error().decode()
+        assert L.gsdf_lowrank_fwd_ws_bytes(C.byref(args)) == 0 and L.gsdf_lowrank_save_bytes(C.byref(args)) == 0 and L.gsdf_lowrank_bwd_ws_bytes(C.byref(args)) == 0
+    for good in (dict(n_adapters=600, n_in=1 << 14, n_out=1 << 14, rank=65), dict(n_adapters=1024, n_in=4096, n_out=4096, rank=64)):      # 3.8e9 and 0.8e9 elements
+        assert L.gsdf_lowrank_fwd_ws_bytes(C.byref(_args(capi, **good))) > 0
+
+
 def test_lowrank_refuses_missing_buffers(capi):
     L, args = capi.lib(), _args(capi)
     assert L.gsdf_lowrank_fwd(None, None, 0, 64, 8, None, 64, None) == -1

@@ -258,6 +258,29 @@ def test_lowrank_in_place(ad, rows):
     assert torch.equal(buf, before)      # the columns beside, the rows behind
 
 
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_lowrank_in_place_beside_its_own_input(ad, rows):
+    """y and x are columns of one buffer: apart they may be, on one another they may not"""
+    x, a, b, ids, scales, base, _ = make(rows, 40, 24, 8, 3, torch.bfloat16, 0.1)
+    want = ref.Lowrank(x, a, b, ids, scales, base)
+    for x0, y0 in ((0, 40), (24, 0), (30, 3)):
+        big = torch.zeros(rows, 72, dtype=x.dtype, device="cuda")
+        big[:, x0:x0 + 40], big[:, y0:y0 + 24] = x, base
+        want.check("y", ad.lowrank_adapt_(big[:, y0:y0 + 24], big[:, x0:x0 + 40], a, b, ids, scales), 48)
+        assert torch.equal(big[:, x0:x0 + 40], x)
+    big = torch.zeros(rows + 1, 72, dtype=x.dtype, device="cuda")
+    for x0, y0 in ((0, 39), (23, 0), (30, 7), (10, 20), (0, 0)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ad.lowrank_adapt_(big[:rows, y0:y0 + 24], big[:rows, x0:x0 + 40], a, b, ids, scales)
+    flat = big.view(-1)
+    with pytest.raises(RuntimeError, match="share memory"):      # rows of different strides
+        ad.lowrank_adapt_(flat[39:39 + rows * 24].view(rows, 24), flat[:rows * 40].view(rows, 40), a, b, ids, scales)
+    if rows == 1:
+        return
+    with pytest.raises(RuntimeError, match="share memory"):      # x is one row, and it lies in y
+        ad.lowrank_adapt_(big[:rows, :24], big[1:2, :40].expand(rows, 40), a, b, ids, scales)
+
+
 def test_lowrank_rows_behind_32_bits(ad):
     """element offsets above 2^32 in x, base, y and dx"""
     rows, stride, k, n = 9, 1 << 29, 72, 40
