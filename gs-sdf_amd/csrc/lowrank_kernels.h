@@ -564,8 +564,8 @@ __device__ __forceinline__ void both_range(const ShrinkArgs &s, const ExpandArgs
   expand_range<T, RT, TT, DROP_Y, RAGGED, PAST, true>(q, range, 0, which % ((q.width + 63) / 64), (q.width + 63) / 64, source);
 }
 template <typename T, int RT, bool DROP_X, bool DROP_Y, bool RAGGED, bool PAST>
-__global__ void __launch_bounds__(256) lowrank_both_kernel(ShrinkArgs s, ExpandArgs q) {
-  const int which = (int)__builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+__global__ void __launch_bounds__(64) lowrank_both_kernel(ShrinkArgs s, ExpandArgs q) {
+  const int which = (int)__builtin_amdgcn_readfirstlane(blockIdx.x);
   if (which >= q.plan.n_wide) return;
   const int4 range = q.plan.wide[which];
   if (range.z == 0 || (range.x == q.plan.n_adapters && q.base == q.y)) return;
@@ -948,14 +948,14 @@ static void products_launch(const Lowrank &q, ShrinkArgs s, ExpandArgs e, bool d
   constexpr int STEP = 128 / (int)sizeof(T), N = 16 / (int)sizeof(T);
   const bool past = (int64_t)q.a.rows * e.width * (int64_t)sizeof(T) >= LR_PAST;
   if (q.both && e.y != nullptr) {
-    const unsigned grid = (unsigned)ceil_div(q.plan.n_wide, 4);
+    const unsigned grid = (unsigned)q.plan.n_wide;
     const bool ragged = s.width % STEP != 0 || e.width % 64 != 0;
     auto run = [&](auto rt, auto dx, auto dy) {
       constexpr int RT = decltype(rt)::value;
       constexpr bool DX = decltype(dx)::value, DY = decltype(dy)::value;
-      if (ragged) lowrank_both_kernel<T, RT, DX, DY, true, false><<<grid, 256, 0, stream>>>(s, e);
-      else if (past) lowrank_both_kernel<T, RT, DX, DY, false, true><<<grid, 256, 0, stream>>>(s, e);
-      else lowrank_both_kernel<T, RT, DX, DY, false, false><<<grid, 256, 0, stream>>>(s, e);
+      if (ragged) lowrank_both_kernel<T, RT, DX, DY, true, false><<<grid, 64, 0, stream>>>(s, e);
+      else if (past) lowrank_both_kernel<T, RT, DX, DY, false, true><<<grid, 64, 0, stream>>>(s, e);
+      else lowrank_both_kernel<T, RT, DX, DY, false, false><<<grid, 64, 0, stream>>>(s, e);
     };
     auto by_drop = [&](auto rt) {
       if (drop_x) run(rt, std::true_type{}, std::false_type{});
