@@ -25,7 +25,7 @@ struct Plan {
   int per, wanted, n_ranges, wide_rows, n_wide, chunk_rows, max_chunks;
 };
 // Every range costs a compute unit about the bytes of its rows and of its adapter's weights, and ends with its adapter: `per` is the smallest size from
-// this one on that makes no more ranges than a multiple of the units (264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 take 20: 8192 rows of 8 KB).
+// this one on that makes no more ranges than a multiple of the units (8192 rows of 8 KB, rank 16: 264 ranges of 32 rows took 28 us on 256 units, 249 of up to 34 took 20).
 // `least`: rows that share the weights at least.  `wide_rows`: rows of a range of `expand`, 16, 32 or 64.
 static size_t plan_layout(Plan *p, void *mem, int64_t rows, int n_adapters, int least, int wide_rows) {
   p->rows = (int)rows; p->n_adapters = n_adapters;

@@ -88,7 +88,8 @@ __device__ __forceinline__ void pack_block(const PackArgs &q, int block) {
 }
 
 // The plan takes two launches: each workgroup counts its share of the rows; then each adds up the counts of all (they are few), finds where its own rows
-// go and puts them there.  Up to 16384 rows each workgroup counts all rows instead, in one launch.
+// go and puts them there.  Up to 16384 rows each workgroup counts all rows instead, in one launch.  A chain of waits, not bytes: 1111 rows of 5 adapters 7.6 us,
+// 8192 of 8 11 us, 300000 of 6 4.7 and 9.4 us.
 __global__ void __launch_bounds__(1024) lowrank_plan_count_kernel(Plan p, Ids ids, PackArgs pack) {
   extern __shared__ int s_hist[];      // [n_adapters + 1]
   if ((int)blockIdx.x >= p.blocks) {

@@ -1,14 +1,20 @@
 // lowrank_kernels.h — the products of the low-rank adapters; lowrank_f32.hip, lowrank_f16.hip and lowrank_bf16.hip compile it for their element type.
 //
 // The adapters' weights are small beside x, base and y, so the operator is bound by the bytes of its rows.  The rows are put in the order of
-// their adapters first (`plan_*`): a tile of 32 rows then has one adapter, and each product is a tile of matrix instructions whose operands
-// come from global memory in the layout that the instruction wants:
+// their adapters first (`lowrank_plan_*`): a range of 16 to 64 rows then has one adapter, and each product is tiles of matrix instructions whose
+// operands come from global memory in the layout that the instruction wants:
 //   shrink   contracts a row's elements (x with A, dy with B^T).  The order of the contraction is free: an instruction's lanes take 64 neighbouring bytes of
 //            each of 16 rows.  The waves of a workgroup split the row and meet in LDS.
 //   expand   contracts ranks (h with B, dh with A^T): the instruction's rows are columns of y, permuted so that a lane holds 16 neighbouring bytes and four lanes 64.
 //   outer    contracts rows (dh with x, h with dy): a lane holds 8 rows x 16 bytes and turns them in registers.
 // h and dh are held in 32 bits.  In front of 16-bit instructions they are split into a high and a low part of the weights' type (16 or 22 bits of the
 // value's), which costs instructions that are not the bound; rounding them once would cost as much precision again as the result's own rounding.
+//
+// Measured beside the bytes that a product cannot do without (a copy of the same size moves 5.2 TB/s):
+//   8192 rows, 4096 -> 4096, rank 16, bf16, dropout: shrink 22 us (64 MB, 3.0 TB/s: the generator's products are half of it; without dropout 18, 3.8 TB/s), expand 32 us
+//     (128 MB, 4.2 TB/s), dx 26 us (64 MB and the generator again), outer 31 us (128 MB, 4.3 TB/s), the sum of its chunks 4 us, plan and layout 11 us (latency)
+//   6007 rows, 4096 -> 4096, rank 64, bf16: shrink 18.5 us, expand 28.6 us (98 MB, 3.4 TB/s: 0.3 GB of weights from the L2 beside them), plan and layout 10.5 us
+//   300000 rows, 64 -> 64, rank 8, 32 bits: both products 53.5 us forward (230 MB, 4.3 TB/s), 43 backward (154 MB, 3.6 TB/s), outer 44 us (173 MB, 3.9 TB/s), sum 5.7 us
 #pragma once
 #include <type_traits>
 
@@ -296,8 +302,8 @@ __global__ void __launch_bounds__(512) lowrank_shrink_kernel(ShrinkArgs q) {
 }
 
 // ---- expand: y[row][n] = base[row][n] + sum_j H[place][j] W[g][n][j] -------------------------------------------------------------------------
-// A wave takes 64 columns of up to 64 rows (the weights come from the L2, whose bandwidth bounds the wider ranks: 32 rows a read took 40 us for a rank of 64
-// where 64 take 3x).  The instruction's rows are columns of y in the order that leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of
+// A wave takes 64 columns of 16, 32 or 64 rows (the weights come from the L2 once for all of them; ranks above 32 stop at 32 rows, whose h leaves room for
+// more waves: rank 64, 6007 rows of 8 KB 28.6 us against 32.6 with 64 rows).  Loads of the next columns are on their way while the last are stored.  The instruction's rows are columns of y in the order that leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of
 // them; lanes of rows c and c + 8 then change pieces, so that an access covers 128 bytes of each of 8 rows instead of 64 of 16 (30 against 34 us for
 // a plain copy of 8192 rows of 8 KB in this manner).
 struct ExpandArgs {
@@ -540,6 +546,7 @@ __global__ void __launch_bounds__(256, RAGGED || RT == 8 ? 1 : 2) lowrank_expand
 }
 
 // ---- both: many rows leave no unit idle when a wave takes a range through `shrink` and `expand` by itself; h stays in its registers -------------
+// Workgroups of one wave: a range is begun as soon as another ends (four waves a workgroup: 55.2 us against 53.7; ranges of 16 rows instead of 32: 61).
 template <typename T, int RT, int TT, bool DROP_X, bool DROP_Y, bool RAGGED, bool PAST>
 __device__ __forceinline__ void both_range(const ShrinkArgs &s, const ExpandArgs &q, int4 range, int which) {
   const int c = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
@@ -576,7 +583,8 @@ __global__ void __launch_bounds__(64) lowrank_both_kernel(ShrinkArgs s, ExpandAr
 }
 
 // ---- outer: sum over an adapter's rows of UT[j][place] V[row][c] ----------------------------------------------------------------------------
-// A workgroup of 8 waves owns a chunk of rows and 16 lanes x 16 bytes of columns; its waves take 32 rows in turn and meet in LDS.
+// A workgroup of 8 waves owns a chunk of rows and 16 lanes x 16 bytes of columns; its waves take 32 rows in turn and meet in LDS.  Chunks of 512 rows instead of
+// 1024 make more workgroups of few columns, but more partial sums: 45 us against 44 for 300000 rows of 64 columns, 33 against 31 for 8192 rows of 4096.
 struct OuterSide {
   const float *ut;      // [..][ut_ld]
   const void *v;
