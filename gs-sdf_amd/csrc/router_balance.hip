@@ -154,8 +154,18 @@ __global__ void __launch_bounds__(1024)
   const int e = t & (width - 1), slice = t / width, slices = 1024 / width;
   double p = 0.0;
   int64_t c = 0;
-  if (e < n_experts)
-    for (int b = slice; b < n_blocks; b += slices) { p += (double)ws.psum[(int64_t)b * n_experts + e]; c += ws.counts[(int64_t)b * n_experts + e]; }
+  if (e < n_experts) {
+    int b = slice;
+    for (; b + 15 * slices < n_blocks; b += 16 * slices) {      // sixteen loads of each on their way together: what this kernel waits for
+      float tp[16];
+      int tc[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { tp[i] = ws.psum[(b + i * slices) * n_experts + e]; tc[i] = ws.counts[(b + i * slices) * n_experts + e]; }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { p += (double)tp[i]; c += tc[i]; }
+    }
+    for (; b < n_blocks; b += slices) { p += (double)ws.psum[b * n_experts + e]; c += ws.counts[b * n_experts + e]; }
+  }
   s_p[t] = p; s_c[t] = c;
   __syncthreads();
   for (int s = slices >> 1; s > 0; s >>= 1) {
