@@ -822,8 +822,9 @@ struct RowArgs {
   const float *scales;
   Dropout drop;
 };
-// h_j of the row, in lane 63 of the wave
-template <typename T>
+// h_j of the row, in lane 63 of the wave.  EIGHT: eight pieces on their way together, then four (48 rows of 4096, rank 32, fp16: 5.1 against 5.4 us; in the
+// one-launch kernel, one row of rank 16, eight took 6.1 us against 5.8)
+template <typename T, bool EIGHT>
 __device__ __forceinline__ float row_rank(const RowArgs &q, const Dropout &drop, int64_t row, int g, int j) {
   typedef typename Vec<T>::vec V;
   constexpr int N = Vec<T>::N;
@@ -836,13 +837,19 @@ __device__ __forceinline__ float row_rank(const RowArgs &q, const Dropout &drop,
     for (int i = 0; i < N; ++i) s = fmaf((float)u[i], (float)v[i], s);
   };
   int k = lane * N;
-  for (; k + 192 * N + N <= width; k += 256 * N) {      // four pieces on their way together
-    V u[4], v[4];
+  auto pieces = [&](auto ahead) {      // pieces on their way together
+    constexpr int AHEAD = decltype(ahead)::value;
+    for (; k + (AHEAD - 1) * 64 * N + N <= width; k += AHEAD * 64 * N) {
+      V u[AHEAD], v[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { u[i] = load_vec<T>(px + k + i * 64 * N); v[i] = load_vec<T>(pa + k + i * 64 * N); }
+      for (int i = 0; i < AHEAD; ++i) { u[i] = load_vec<T>(px + k + i * 64 * N); v[i] = load_vec<T>(pa + k + i * 64 * N); }
+      if (EIGHT) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) add(k + i * 64 * N, u[i], v[i]);
-  }
+      for (int i = 0; i < AHEAD; ++i) add(k + i * 64 * N, u[i], v[i]);
+    }
+  };
+  if (EIGHT) pieces(std::integral_constant<int, 8>{});
+  pieces(std::integral_constant<int, 4>{});
   for (; k + N <= width; k += 64 * N) add(k, load_vec<T>(px + k), load_vec<T>(pa + k));
   if (k < width) add(k, load_vec_end<T>(px, k, width), load_vec_end<T>(pa, k, width));
   return wave_sum_to_lane63(s) * (q.scales != nullptr ? q.scales[g] : 1.f) * (drop.threshold != 0 ? drop.scale : 1.f);
@@ -857,22 +864,31 @@ __device__ __forceinline__ void row_columns(const RowArgs &q, int64_t row, int g
   const T *base = (const T *)q.base + row * q.base_stride, *pb = (const T *)q.b + (int64_t)g * q.n_out * rank;
   T *y = (T *)q.y + row * q.y_stride;
   constexpr int C = 4;      // columns on their way together
-  for (; n < q.n_out; n += C * step) {
-    float v[C], s[C];
+  float v[C];
+  V w[C];
+  auto weights = [&](int j) {      // of ranks j .. j + N
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const T *p = pb + (int64_t)(n + c * step < q.n_out ? n + c * step : n) * rank;
+      w[c] = j + N <= rank ? load_vec<T>(p + j) : load_vec_end<T>(p, j, rank);
+    }
+  };
+  auto begin = [&]() {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int at = n + c * step;
       v[c] = q.base != nullptr && at < q.n_out ? (float)base[at] : 0.f;
-      s[c] = 0.f;
     }
+    if (has && sub * N < rank) weights(sub * N);
+  };
+  if (n < q.n_out) begin();
+  while (n < q.n_out) {
+    float s[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) s[c] = 0.f;
     if (has) {
       for (int j = sub * N; j < rank; j += LPC * N) {
-        V w[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const T *p = pb + (int64_t)(n + c * step < q.n_out ? n + c * step : n) * rank;
-          w[c] = j + N <= rank ? load_vec<T>(p + j) : load_vec_end<T>(p, j, rank);
-        }
+        if (j != sub * N) weights(j);
         float t[N];
         if (j + N <= rank) {
 #pragma unroll
@@ -897,6 +913,8 @@ __device__ __forceinline__ void row_columns(const RowArgs &q, int64_t row, int g
       for (int o = 1; o < LPC; o <<= 1) s[c] += __shfl_xor(s[c], o);
       if (sub == 0 && n + c * step < q.n_out) y[n + c * step] = (T)(s[c] + v[c]);
     }
+    n += C * step;
+    if (n < q.n_out) begin();
   }
 }
 template <typename T>
@@ -913,7 +931,7 @@ __global__ void __launch_bounds__(1024) lowrank_row_shrink_kernel(RowArgs q) {
   const int j = blockIdx.y * 16 + (threadIdx.x >> 6), g = group_of(q.ids, row);
   if (j >= q.rank || g == q.ids.n_adapters) return;
   dropout_counter(q.drop);
-  const float v = row_rank<T>(q, q.drop, row, g, j);
+  const float v = row_rank<T, true>(q, q.drop, row, g, j);
   if ((threadIdx.x & 63) == 63) q.h[row * q.rank + j] = v;
 }
 template <typename T>
@@ -933,7 +951,7 @@ __global__ void __launch_bounds__(1024) lowrank_row_kernel(RowArgs q) {
   if (g < q.ids.n_adapters) {
     dropout_counter(q.drop);
     for (int j = threadIdx.x >> 6; j < q.rank; j += 16) {
-      const float v = row_rank<T>(q, q.drop, row, g, j);
+      const float v = row_rank<T, false>(q, q.drop, row, g, j);
       if ((threadIdx.x & 63) == 63) s_h[j] = v;
     }
   }
