@@ -234,7 +234,7 @@ __device__ __forceinline__ void shrink_sums(const ShrinkArgs &q, int4 range, int
   if (RT == 1 && TT < 3) steps(std::integral_constant<int, 4>{});
   if (RT <= 4) steps(std::integral_constant<int, 2>{});
   steps(std::integral_constant<int, 1>{});
-  if (RAGGED && part == full % q.split) {      // the rows' last elements
+  if (RAGGED && full * STEP < q.width && part == full % q.split) {      // the rows' last elements (RAGGED may be for y's width alone)
     const int k = full * STEP + quad * N;
     V xs[TT][2], ws[RT][2];
 #pragma unroll

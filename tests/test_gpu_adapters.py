@@ -207,6 +207,52 @@ def test_lowrank_infinities_stay_in_their_rows_and_adapters(ad, rows, dtype):
     assert not torch.isfinite(y[2].float()).any() and not torch.isfinite(da[2].float()).any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 64, 64, 16, 1), (5, 33, 70, 20, 3), (48, 256, 128, 32, 4), (300, 41, 23, 12, 3), (300, 128, 64, 8, 9), (700, 264, 1024, 100, 2), (3000, 64, 40, 8, 5),
+                                   (20000, 24, 64, 64, 7), (65567, 8, 128, 24, 200), (65567, 128, 8, 24, 200), (66000, 64, 64, 8, 6), (66000, 72, 100, 4, 3), (66000, 128, 64, 7, 3)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_lowrank_reads_nothing_it_did_not_write(ad, shape, dtype):
+    """the saved buffer, the workspaces and what lies behind them hold NaN: the results are those of buffers of zeros"""
+    import ctypes as C
+    from gs_sdf_amd import capi
+    L, (rows, k, n, r, g) = capi.lib(), shape
+    x, a, b, ids, scales, base, dy = make(rows, k, n, r, g, dtype, 0.1, rows > 20000)
+    d = dict(rows=rows, x_stride=k, n_in=k, n_out=n, rank=r, n_adapters=g, dtype=DTYPES.index(dtype), ids_64=0, x=x.data_ptr(), a=a.data_ptr(), b=b.data_ptr(), ids=ids.data_ptr(),
+             scales=scales.data_ptr(), p=0.1, seed=1, offset=2, offset_dev=None)
+    args = C.byref(capi.LowrankArgs(*[d[name] for name, _ in capi.LowrankArgs._fields_]))
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    got = []
+    for fill in (0, 255):
+        hold = lambda size: torch.full((size + 65536,), fill, dtype=torch.uint8, device="cuda")  # noqa: E731
+        save, ws, wb = hold(L.gsdf_lowrank_save_bytes(args)), hold(L.gsdf_lowrank_fwd_ws_bytes(args)), hold(L.gsdf_lowrank_bwd_ws_bytes(args))
+        y, alone, dx, da, db = (torch.full_like(t, math.nan) for t in (base, base, x, a, b))
+        assert L.gsdf_lowrank_fwd(args, base.data_ptr(), n, y.data_ptr(), n, save.data_ptr(), ws.data_ptr(), stream) == 0
+        assert L.gsdf_lowrank_bwd(args, dy.data_ptr(), n, save.data_ptr(), dx.data_ptr(), k, da.data_ptr(), db.data_ptr(), wb.data_ptr(), stream) == 0
+        assert L.gsdf_lowrank_fwd(args, base.data_ptr(), n, alone.data_ptr(), n, None, hold(L.gsdf_lowrank_fwd_ws_bytes(args)).data_ptr(), stream) == 0
+        torch.cuda.synchronize()
+        got.append((y, alone, dx, da, db))
+    for u, v in zip(*got):
+        assert torch.isfinite(u).all() and torch.equal(u, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("k,n", [(8, 128), (128, 8), (64, 72)])
+def test_lowrank_infinities_of_many_rows_stay_in_their_adapters(ad, k, n, dtype):
+    x, a, b, ids, scales, base, dy = make(65600, k, n, 8, 3, dtype, 0.05)
+    want = ref.Lowrank(x, a[:2], b[:2], torch.where(ids == 2, -1, ids), scales[:2], base, dy)
+    a[2], b[2] = math.inf, math.inf
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = ad.lowrank_adapt(x, a, b, ids, scales, base)
+    dx, da, db = torch.autograd.grad(y, leaves, dy)
+    ok = (ids != 2).cpu()
+    for name, t in (("y", y), ("dx", dx)):
+        for suffix in ("", "_mag", "_split"):
+            setattr(want, name + suffix, getattr(want, name + suffix)[ok])
+        want.check(name, t[ok.cuda()], k + n)
+    want.check("da", da[:2], n + 65600)
+    want.check("db", db[:2], k + 65600)
+
+
 def test_lowrank_dropped_infinities_are_gone(ad):
     x, a, b, ids, scales, base, dy = make(64, 80, 40, 8, 2, torch.bfloat16)
     f = ref.keep_factor(64, 80, 0.5, 11, 3)
