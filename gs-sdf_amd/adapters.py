@@ -43,8 +43,8 @@ def _ops():
 def lowrank_adapt(x, a, b, ids, scales=None, base=None, p=0.0, seed=0, offset=0):
     """y = base + s_g B_g A_g drop(x) for every row, g = ids[row]: x [..., k], a [g, r, k], b [g, n, r], ids [...] (int32 / int64), scales [g] fp32
     constants (None: 1), base [..., n] (None: 0) -> y [..., n].  A row whose id is outside [0, g) has no adapter: y is base there.  p > 0 drops elements of
-    x as dropout(x, p, seed, offset) would.  Gradients for x, a, b and base (once; a rank up to 128, up to 1024 adapters).  Beside 16-bit elements h is held as
-    a sum of two of them: where a factor is infinite the result is not finite, but may be NaN where the formula has an infinity."""
+    x as dropout(x, p, seed, offset) would.  Gradients for x, a, b and base (once; a rank up to 128, up to 1024 adapters).  h keeps its 32 bits beside
+    16-bit elements, as a sum of three of them: where a factor is infinite the result is not finite, but may be NaN where the formula has an infinity."""
     return (_mod or _ops()).lowrank_adapt(x, a, b, ids, scales, base, p, seed, offset)
 
 

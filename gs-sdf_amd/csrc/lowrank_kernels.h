@@ -7,8 +7,8 @@
 //            each of 16 rows.  The waves of a workgroup split the row and meet in LDS.
 //   expand   contracts ranks (h with B, dh with A^T): the instruction's rows are columns of y, permuted so that a lane holds 16 neighbouring bytes and four lanes 64.
 //   outer    contracts rows (dh with x, h with dy): a lane holds 8 rows x 16 bytes and turns them in registers.
-// h and dh are held in 32 bits.  In front of 16-bit instructions they are split into a high and a low part of the weights' type (16 or 22 bits of the
-// value's), which costs instructions that are not the bound; rounding them once would cost as much precision again as the result's own rounding.
+// h and dh are held in 32 bits.  In front of 16-bit instructions they are split into three parts of the weights' type, which hold all 24 bits between
+// them: the instructions are not the bound.
 //
 // Measured beside the bytes that a product cannot do without (a copy of the same size moves 5.2 TB/s):
 //   8192 rows, 4096 -> 4096, rank 16, bf16, dropout: shrink 22 us (64 MB, 3.0 TB/s: the generator's products are half of it; without dropout 18, 3.8 TB/s), expand 32 us
@@ -148,16 +148,28 @@ __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 acc) {
   for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
   return acc;
 }
-// what rounding v to h left; an infinity leaves nothing
-template <typename T>
-__device__ __forceinline__ T low_part(float v, T h) {
-  return fabsf((float)h) == INFINITY ? (T)0.f : (T)(v - (float)h);
+// v = hi + mid + lo: eight bits each, cut off and not rounded, so that no part of a finite number is infinite (bf16); eleven (fp16).  An infinity leaves nothing.
+__device__ __forceinline__ void split(float v, bf16_t &hi, bf16_t &mid, bf16_t &lo) {
+  auto top = [](float t) { return __float_as_uint(t) & 0xFFFF0000u; };
+  auto part = [](uint32_t t) { return __builtin_bit_cast(bf16_t, (unsigned short)(t >> 16)); };
+  const uint32_t h = top(v);
+  const float r = fabsf(v) == INFINITY ? 0.f : v - __uint_as_float(h);
+  const uint32_t m = top(r);
+  hi = part(h); mid = part(m); lo = part(top(r - __uint_as_float(m)));
 }
-// a power of two that brings `largest` into [1, 2): 16-bit numbers of fp16 would run over or vanish
-__device__ __forceinline__ float scale_to_one(float largest) {
-  const int e = (__float_as_int(largest) >> 23) & 255;
-  return e == 0 || e == 255 ? 1.f : __int_as_float((254 - e < 1 ? 1 : 254 - e) << 23);
+__device__ __forceinline__ void split(float v, f16_t &hi, f16_t &mid, f16_t &lo) {
+  hi = (f16_t)v;
+  const float r = fabsf((float)hi) == INFINITY ? 0.f : v - (float)hi;
+  mid = (f16_t)r;
+  lo = (f16_t)(r - (float)mid);
 }
+// In front of fp16 parts: a power of two that brings `largest` into [2^14, 2^15), where neither it nor what is 2^38 times smaller runs over or vanishes;
+// times `scale_back` of it everything is as before.  Infinities and what is all zeros stay.
+__device__ __forceinline__ float scale_up(float largest) {
+  const int e = (__float_as_int(largest) >> 23) & 255, up = 268 - e;
+  return e == 0 || e == 255 ? 1.f : __int_as_float((up < 253 ? up : 253) << 23);
+}
+__device__ __forceinline__ float scale_back(float scale) { return __int_as_float((254 << 23) - __float_as_int(scale)); }
 
 // ---- shrink: H[place][j] = factor sum_k drop(x)[row][k] W[g][j][k] -------------------------------------------------------------------------
 // A workgroup of `split` waves has a range of rows and its waves take the steps of 128 bytes in turn (one wave: four ranges a workgroup).
@@ -329,7 +341,8 @@ __device__ __forceinline__ void change_halves(V &a_, V &b_, bool upper) {
   b_ = __builtin_bit_cast(V, b);
 }
 // HERE: h comes from the wave's own sums, whose layout (a lane has 4 ranks of its row) an instruction takes as it is when the ranks of the contraction
-// are told the weights in that order: four high and four low parts a lane at 16 bits.  Else it is read from H.  `source` fills f.
+// are told the weights in that order: four ranks' first and second parts a lane at 16 bits, and their third beside zeros.  Else it is read from H.  `source`
+// fills f.
 template <typename T, int RT, int TT, bool DROP, bool RAGGED, bool PAST, bool HERE, typename Source>
 __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, int part, int turn, int chunks, Source source) {
   typedef typename Vec<T>::vec V;
@@ -382,9 +395,9 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
     return;
   }
   const T *w = (const T *)q.w + range.x * q.w_group;
-  // h of the lane's row as the instruction wants it.  16 bits: 8 ranks a lane, 32 an instruction, high and low parts (a rank of at most 16: both in
+  // h of the lane's row as the instruction wants it.  16 bits: 8 ranks a lane, 32 an instruction, one for each part (a rank of at most 16: two parts in
   // one instruction).  32 bits: 4 ranks a lane, 16 a group of four instructions.
-  constexpr bool BOTH = !WIDE && (HERE || RT == 1);      // high and low parts in one instruction
+  constexpr bool BOTH = !WIDE && (HERE || RT == 1);      // first and second parts in one instruction
   constexpr int KB = WIDE || HERE ? RT : (RT == 1 ? 1 : RT / 2), FN = WIDE || HERE ? 1 : 2;
   auto rank_of = [&](int k) { return WIDE || HERE ? k * 16 + quad * 4 : (RT == 1 ? (quad & 1) * 8 : k * 32 + quad * 8); };
   V b[2 * TT][NP], u[4][KB];
@@ -411,7 +424,7 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
   auto chunk_of = [&](int i) { return i + turn < chunks ? i + turn : i + turn - chunks; };
   load_weights(chunk_of(part));
   load_base(chunk_of(part), b);
-  V hi[TT][KB], lo[TT][KB];
+  V hi[TT][KB], mid[TT][KB], lo[TT][KB];
   float back[TT];
   uint32_t row_of[TT];
   f32x4 f[TT][KB][FN];
@@ -428,27 +441,32 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
 #pragma unroll
         for (int l = 0; l < 4; ++l) largest = fmaxf(largest, fabsf(f[t][k][e][l]));
       }
-    float down = 1.f;
+    float scale = 1.f;
     back[t] = 1.f;
     if (__is_same(T, f16_t)) {
       largest = fmaxf(largest, __shfl_xor(largest, 16));
       largest = fmaxf(largest, __shfl_xor(largest, 32));
-      down = scale_to_one(largest);
-      back[t] = 1.f / down;
+      scale = scale_up(largest);
+      back[t] = scale_back(scale);
     }
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
       for (int e = 0; e < FN * 4; ++e) {
-        const float v = f[t][k][e / 4][e % 4] * down;
-        const T h = (T)v;
-        const T l = low_part<T>(v, h);
-        if constexpr (HERE && !WIDE) {
-          hi[t][k][e] = h;
-          hi[t][k][e + 4] = l;
+        const float v = f[t][k][e / 4][e % 4] * scale;
+        if constexpr (WIDE) {
+          hi[t][k][e] = v;
         } else {
-          hi[t][k][e] = BOTH && quad >= 2 ? l : h;
-          lo[t][k][e] = l;
+          T h, m, l;
+          split(v, h, m, l);
+          if (HERE) {
+            hi[t][k][e] = h; hi[t][k][e + 4] = m;
+            lo[t][k][e] = l; lo[t][k][e + 4] = (T)0.f;
+          } else {
+            hi[t][k][e] = BOTH && quad >= 2 ? m : h;
+            mid[t][k][e] = m;
+            lo[t][k][e] = BOTH && quad >= 2 ? (T)0.f : l;
+          }
         }
       }
   }
@@ -467,8 +485,9 @@ __device__ __forceinline__ void expand_range(const ExpandArgs &q, int4 range, in
         acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
+          if (!WIDE) acc[m] = mma(u[m][k], lo[t][k], acc[m]);
+          if (!WIDE && !BOTH) acc[m] = mma(u[m][k], mid[t][k], acc[m]);
           acc[m] = mma(u[m][k], hi[t][k], acc[m]);
-          if (!WIDE && !BOTH) acc[m] = mma(u[m][k], lo[t][k], acc[m]);
         }
       }
 #pragma unroll
@@ -688,7 +707,7 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
           for (int i = 0; i < 8; ++i) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[r][i / 4][i % 4], v[i][e], acc[r][e], 0, 0, 0);
     } else {
       constexpr bool HALF = __is_same(T, f16_t);
-      float down = 1.f, up = 1.f;
+      float scale = 1.f, back = 1.f;
       if (HALF) {      // one power of two for the step: the sums of other steps keep their own
         float largest = 0.f;
 #pragma unroll
@@ -697,17 +716,17 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
           for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(u[r][i / 4][i % 4]));
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o));
-        down = scale_to_one(largest);
-        up = 1.f / down;
+        scale = scale_up(largest);
+        back = scale_back(scale);
       }
-      V hi[RT], lo[RT];
+      V hi[RT], mid[RT], lo[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float t = u[r][i / 4][i % 4] * down;
-          hi[r][i] = (T)t;
-          lo[r][i] = low_part<T>(t, hi[r][i]);
+          T h, m, l;
+          split(u[r][i / 4][i % 4] * scale, h, m, l);
+          hi[r][i] = h; mid[r][i] = m; lo[r][i] = l;
         }
       u32x4 words[8];
 #pragma unroll
@@ -719,11 +738,13 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
         for (int r = 0; r < RT; ++r) {
           if (HALF) {
             f32x4 t = mma(lo[r], b, f32x4{0.f, 0.f, 0.f, 0.f});
+            t = mma(mid[r], b, t);
             t = mma(hi[r], b, t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[r][e][i] = fmaf(t[i], up, acc[r][e][i]);
+            for (int i = 0; i < 4; ++i) acc[r][e][i] = fmaf(t[i], back, acc[r][e][i]);
           } else {
             acc[r][e] = mma(lo[r], b, acc[r][e]);
+            acc[r][e] = mma(mid[r], b, acc[r][e]);
             acc[r][e] = mma(hi[r], b, acc[r][e]);
           }
         }

@@ -1,0 +1,84 @@
+"""The adapter operators (gs_sdf_amd.adapters) at their edges, on the GPU: inner values that need all 32 bits, ranks of very different sizes, what a call has to
+refuse before it writes, derivatives of other kinds than one backward pass."""
+import math
+
+import pytest
+import torch
+
+import adapters_ref as ref
+from test_gpu_adapters import make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ad():
+    from gs_sdf_amd import adapters
+    return adapters
+
+
+def whole_numbers(dtype, rows, width, gen, *lead):
+    """[*lead, rows, width] whole numbers of the type whose products, summed over `width`, need 24 bits and fit them: every 32-bit sum of them is exact"""
+    lo, hi = (128, 255) if dtype == torch.bfloat16 else (1200, 1448)
+    return torch.randint(lo, hi + 1, (*lead, rows, width), generator=gen).double()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["float16", "bfloat16"])
+@pytest.mark.parametrize("rows,r", [(40, 8), (300, 2), (300, 16), (300, 24), (700, 64), (900, 128), (65600, 4), (65600, 16), (65600, 32)])
+def test_lowrank_inner_values_keep_32_bits(ad, rows, r, dtype):
+    """h (dh) of 24 bits whose last digits alone are left: neighbouring ranks differ by x[., 0] (dy[., 0]) and are taken from one another, and so are neighbouring
+    rows in the weights' gradients.  All sums are whole numbers below 2^24 and the results fit the type: they are equal, not close."""
+    gen = torch.Generator().manual_seed(rows + r)
+    wide, n, g = 256 if dtype == torch.bfloat16 else 8, 72, 3
+    ids = torch.randint(-1, g, (rows // 2,), generator=gen).repeat_interleave(2)      # pairs of rows share an adapter
+    rich = whole_numbers(dtype, rows, wide, gen)
+    rich[1::2] = rich[0::2]
+    rich[1::2, 0] -= 1
+    weights = whole_numbers(dtype, r, wide, gen, g)
+    weights[:, 1::2] = weights[:, 0::2]
+    weights[:, 1::2, 0] -= 1
+    rich[:, 0], weights[:, :, 0] = rich[:, 0].clamp(min=130 if wide == 256 else 1202), weights[:, :, 0].clamp(max=254 if wide == 256 else 1447)
+    rich[1::2, 0] = rich[0::2, 0] - 1
+    weights[:, 1::2, 0] = weights[:, 0::2, 0] - 1
+    pick = torch.zeros(g, n, r, dtype=torch.float64)      # column i takes the two ranks of pair i mod r / 2 from one another
+    for i in range(n):
+        pick[:, i, 2 * (i % (r // 2))], pick[:, i, 2 * (i % (r // 2)) + 1] = 1, -1
+    pairs = torch.zeros(rows, n, dtype=torch.float64)     # column i takes the two rows of pair i from one another
+    for i in range(min(n, rows // 2)):
+        pairs[2 * i, i], pairs[2 * i + 1, i] = 1, -1
+    on = (ids >= 0).double()[:, None]
+    first = torch.zeros(g, n, dtype=torch.float64)        # the adapter of pair i
+    for i in range(min(n, rows // 2)):
+        if ids[2 * i] >= 0:
+            first[ids[2 * i], i] = 1
+    d = lambda t: t.to(dtype).cuda().requires_grad_(True)  # noqa: E731
+    assert float((rich[:64] @ weights[0].T).max()) < 2 ** 24 and float((rich[:64] @ weights[0].T).max()) > 2 ** 23
+    x, a, b, dy, ids = d(rich), d(weights), d(pick), d(pairs), ids.to(torch.int32).cuda()
+    y = ad.lowrank_adapt(x, a, b, ids)
+    assert torch.equal(y.detach().cpu().double(), (rich[:, :1] * on).expand(rows, n))
+    db, = torch.autograd.grad(y, b, dy)      # h of row 2 i less h of row 2 i + 1: a[., 0]
+    assert torch.equal(db.cpu().double(), first[:, :, None] * weights[:, None, :, 0])
+    x, a, b, dy = d(pairs), d(pick.transpose(1, 2)), d(weights.transpose(1, 2)), d(rich)
+    y = ad.lowrank_adapt(x, a, b, ids)
+    dx, da = torch.autograd.grad(y, (x, a), dy)
+    assert torch.equal(dx.cpu().double(), (rich[:, :1] * on).expand(rows, n))
+    assert torch.equal(da.cpu().double(), first[:, None, :] * weights[:, :, :1])
+
+
+def check_alone(want, name, got, terms, rank_dim=None, ranks=None):
+    """as Lowrank.check, but nothing is allowed for values that do not take part in an element's own sum: what is left of the split of h is 2^-38 of the largest h"""
+    w, mag, split = getattr(want, name), getattr(want, name + "_mag"), getattr(want, name + "_split")
+    if rank_dim is not None:
+        at = torch.tensor(ranks)
+        got, w, mag, split = got.index_select(rank_dim, at.to(got.device)), w.index_select(rank_dim, at), mag.index_select(rank_dim, at), 0.0
+    ref.within(got, w, ref.HALF[got.dtype] * w.abs() + (1 + ref.HALF[got.dtype]) * ((3 * terms + 16) * 2.0 ** -24 * mag + 2.0 ** -38 * split), name, got.dtype)
+
+
+@pytest.mark.parametrize("rows,r", [(300, 12), (300, 24), (700, 64), (65600, 16)])
+def test_lowrank_small_ranks_in_a_row_of_large_ones(ad, rows, r):
+    """fp16: y from a rank whose h is 3e-7 of another's, which has no part in y"""
+    x, a, b, ids, scales, base, _ = make(rows, 64, 72, r, 3, torch.float16, 0.1)
+    a[:, 0] *= 1e4
+    b[:, :, 0] = 0
+    a[:, 1:] *= 2e-3
+    check_alone(ref.Lowrank(x, a, b, ids, scales), "y", ad.lowrank_adapt(x.requires_grad_(True), a, b, ids, scales), 64 + r)
