@@ -647,6 +647,20 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int e = 0; e < VE; ++e) acc[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // fp16: the power of two in front of the split of rank c of a tile, and of its sums until the waves meet.  One for each rank: an infinity, or values that are far
+  // larger, are nothing to the others.  It comes down where a step has more (with room for four times as much).
+  constexpr bool HALF = __is_same(T, f16_t);
+  float scale[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) scale[r] = __int_as_float(253 << 23);
+  auto times_of_ranks = [&](f32x4 (&v)[VE], float f) {      // a lane's sums are of ranks quad * 4 ..
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float t = __shfl(f, quad * 4 + i);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e][i] *= t;
+    }
+  };
   const int steps = (chunk.z + 31) / 32;
   const int *order = q.plan.order + chunk.y;
   const bool columns_whole = !RAGGED || col0 + COLS <= s.width;
@@ -706,18 +720,27 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[r][i / 4][i % 4], v[i][e], acc[r][e], 0, 0, 0);
     } else {
-      constexpr bool HALF = __is_same(T, f16_t);
-      float scale = 1.f, back = 1.f;
-      if (HALF) {      // one power of two for the step: the sums of other steps keep their own
-        float largest = 0.f;
+      if (HALF) {
+        float fresh[RT];
+        bool any = false;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r) {
+          float largest = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(u[r][i / 4][i % 4]));
+          largest = fmaxf(largest, __shfl_xor(largest, 16));
+          largest = fmaxf(largest, __shfl_xor(largest, 32));
+          const bool more = largest * scale[r] >= 32768.f && largest != INFINITY;
+          fresh[r] = more ? 0.25f * scale_up(largest) : scale[r];
+          any |= more;
+        }
+        if (__any(any)) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o));
-        scale = scale_up(largest);
-        back = scale_back(scale);
+          for (int r = 0; r < RT; ++r) {
+            times_of_ranks(acc[r], fresh[r] * scale_back(scale[r]));
+            scale[r] = fresh[r];
+          }
+        }
       }
       V hi[RT], mid[RT], lo[RT];
 #pragma unroll
@@ -725,7 +748,7 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           T h, m, l;
-          split(u[r][i / 4][i % 4] * scale, h, m, l);
+          split(HALF ? u[r][i / 4][i % 4] * scale[r] : u[r][i / 4][i % 4], h, m, l);
           hi[r][i] = h; mid[r][i] = m; lo[r][i] = l;
         }
       u32x4 words[8];
@@ -736,20 +759,16 @@ __global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
         const V b = __builtin_bit_cast(V, column_of(words, e));
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          if (HALF) {
-            f32x4 t = mma(lo[r], b, f32x4{0.f, 0.f, 0.f, 0.f});
-            t = mma(mid[r], b, t);
-            t = mma(hi[r], b, t);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[r][e][i] = fmaf(t[i], back, acc[r][e][i]);
-          } else {
-            acc[r][e] = mma(lo[r], b, acc[r][e]);
-            acc[r][e] = mma(mid[r], b, acc[r][e]);
-            acc[r][e] = mma(hi[r], b, acc[r][e]);
-          }
+          acc[r][e] = mma(lo[r], b, acc[r][e]);
+          acc[r][e] = mma(mid[r], b, acc[r][e]);
+          acc[r][e] = mma(hi[r], b, acc[r][e]);
         }
       }
     }
+  }
+  if (HALF) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) times_of_ranks(acc[r], scale_back(scale[r]));
   }
   // the waves' sums: 4 + 4, 2 + 2, 1 + 1, one tile of ranks at a time
 #pragma unroll

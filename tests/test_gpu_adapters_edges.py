@@ -9,6 +9,8 @@ import adapters_ref as ref
 from test_gpu_adapters import make
 
 pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+IDS = [str(d).split(".")[1] for d in DTYPES]
 
 
 @pytest.fixture(scope="module")
@@ -74,6 +76,26 @@ def check_alone(want, name, got, terms, rank_dim=None, ranks=None):
     ref.within(got, w, ref.HALF[got.dtype] * w.abs() + (1 + ref.HALF[got.dtype]) * ((3 * terms + 16) * 2.0 ** -24 * mag + 2.0 ** -38 * split), name, got.dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,r", [(300, 12), (300, 24), (700, 64), (900, 100), (65600, 16)])
+def test_lowrank_small_ranks_beside_large_ones(ad, rows, r, dtype):
+    """a rank whose h and dh are 1e-5 of the others' keeps its own digits in the weights' gradients"""
+    x, a, b, ids, scales, base, dy = make(rows, 64, 72, r, 3, dtype, 0.1)
+    small = [1, r - 3]
+    with torch.no_grad():
+        a[:, small] *= 2e-5
+        b[:, :, small] *= 2e-5
+        if dtype != torch.float32:
+            x *= 4.0
+            dy *= 4.0
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    want = ref.Lowrank(x, a, b, ids, scales, base, dy)
+    dx, da, db = torch.autograd.grad(ad.lowrank_adapt(x, a, b, ids, scales, base), leaves, dy)
+    check_alone(want, "da", da, 72 + rows, 1, small)
+    check_alone(want, "db", db, 64 + rows, 2, small)
+    check_alone(want, "dx", dx, 72 + r)
+
+
 @pytest.mark.parametrize("rows,r", [(300, 12), (300, 24), (700, 64), (65600, 16)])
 def test_lowrank_small_ranks_in_a_row_of_large_ones(ad, rows, r):
     """fp16: y from a rank whose h is 3e-7 of another's, which has no part in y"""
@@ -82,3 +104,27 @@ def test_lowrank_small_ranks_in_a_row_of_large_ones(ad, rows, r):
     b[:, :, 0] = 0
     a[:, 1:] *= 2e-3
     check_alone(ref.Lowrank(x, a, b, ids, scales), "y", ad.lowrank_adapt(x.requires_grad_(True), a, b, ids, scales), 64 + r)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,r", [(300, 12), (300, 24), (700, 64), (900, 100), (65600, 16)])
+def test_lowrank_an_infinity_in_one_rank_stays_there(ad, rows, r, dtype):
+    """an infinite weight of one rank: the gradients of the others are what they are without that rank, above the largest fp16 number too"""
+    x, a, b, ids, scales, base, dy = make(rows, 64, 72, r, 3, dtype, 0.1)
+    few = 2e-3 if rows < 1000 else 2e-4      # (sums of all rows that fit the type)
+    x, dy, b = x * few, dy * 400, b * 60
+    keep = [i for i in range(r) if i != 2]
+    want = ref.Lowrank(x, a, b, ids, scales, base, dy)
+    b[1, 5, 2] = math.inf
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    da, = torch.autograd.grad(ad.lowrank_adapt(x, a, b, ids, scales, base), leaves[1:2], dy)
+    assert not torch.isfinite(da[1, 2].float()).any()
+    check_alone(want, "da", da, 72 + rows, 1, keep)
+    x, a, b, ids, scales, base, dy = make(rows, 64, 72, r, 3, dtype, 0.1)
+    x, a, dy = x * 400, a * 200, dy * few
+    want = ref.Lowrank(x, a, b, ids, scales, base, dy)
+    a[1, 2, 7] = -math.inf
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    db, = torch.autograd.grad(ad.lowrank_adapt(x, a, b, ids, scales, base), leaves[2:], dy)
+    assert not torch.isfinite(db[1, :, 2].float()).any()
+    check_alone(want, "db", db, 64 + rows, 2, keep)
