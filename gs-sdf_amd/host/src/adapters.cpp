@@ -55,6 +55,11 @@ void check_word(const Tensor &ref, const Offset &offset) {
 }
 gsdf_stream_t stream_of(const Tensor &t) { return (gsdf_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 bool wanted(const Tensor &t) { return t.defined() && t.requires_grad(); }
+// a dual tensor asks for no gradient: its tangent would be lost without an error
+void no_tangents(const char *name, std::initializer_list<const Tensor *> inputs) {
+  for (const Tensor *t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, ": no forward-mode derivatives (an input has a tangent)");
+}
 void *at_or_null(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(const Tensor &ref, size_t n) { return torch::empty({(int64_t)n}, ref.options().dtype(torch::kUInt8).requires_grad(false)); }
 Tensor plain(const Tensor &ref, at::IntArrayRef shape) { return torch::empty(shape, ref.options().requires_grad(false)); }
@@ -123,6 +128,7 @@ struct LowrankFunction : public torch::autograd::Function<LowrankFunction> {
     if (!dy.defined()) return variable_list(5);
     LowrankCall c{s[3], s[4], s[5], (int)ctx->saved_data["dtype"].toInt(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(),
                   (uint64_t)ctx->saved_data["offset"].toInt()};
+    no_tangents("lowrank_adapt's backward pass", {&dy});
     const bool need_x = ctx->needs_input_grad(0), need_a = ctx->needs_input_grad(1), need_b = ctx->needs_input_grad(2),
                need_base = ctx->saved_data["base"].toBool() && ctx->needs_input_grad(3);
     const Tensor dx = need_x ? plain(x, x.sizes()) : Tensor(), da = need_a ? plain(a, a.sizes()) : Tensor(), db = need_b ? plain(b, b.sizes()) : Tensor();
@@ -155,6 +161,7 @@ LowrankCall lowrank_check(const Tensor &x, Tensor &a, Tensor &b, const Tensor &i
   if (scales) {
     same(x, *scales, "scales", torch::kFloat32);
     TORCH_CHECK(scales->dim() == 1 && scales->size(0) == a.size(0), "scales: expected shape [", a.size(0), "], got ", scales->sizes());
+    no_tangents("lowrank_adapt", {&*scales});
     TORCH_CHECK(!(scales->requires_grad() && torch::GradMode::is_enabled()), "scales: constants, no gradient is offered for them");
     c.scales = whole(*scales);
   }
@@ -167,6 +174,7 @@ LowrankCall lowrank_check(const Tensor &x, Tensor &a, Tensor &b, const Tensor &i
   check_word(x, offset);
   c.p = p; c.seed = seed; c.offset = offset.number;
   if (offset.word) c.word = *offset.word;
+  no_tangents("lowrank_adapt", {&x, &a, &b, &base});
   a = whole(a);
   b = whole(b);
   return c;
@@ -213,6 +221,7 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor &dy = grads[0];
     if (!dy.defined()) return variable_list(3);
+    no_tangents("dropout's backward pass", {&dy});
     const DropoutCall c{ctx->get_saved_variables()[0], (int)ctx->saved_data["dtype"].toInt(), ctx->saved_data["p"].toDouble(),
                         (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()};
     return once("dropout", {ctx->needs_input_grad(0) ? dropout_run(dy, Tensor(), c) : Tensor(), ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? dy : Tensor(), Tensor()});
@@ -250,6 +259,7 @@ struct BalanceFunction : public torch::autograd::Function<BalanceFunction> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &m = s[0], &mask = s[1], &pull = s[2];
     if (!grads[0].defined()) return variable_list(2);
+    no_tangents("router_balance's backward pass", {&grads[0]});
     const c10::DeviceGuard guard(m.device());
     const Tensor v = grads[0].to(torch::kFloat32).contiguous(), out = plain(m, {m.size(0), m.size(1)});
     check(gsdf_router_balance_bwd(m.size(0), (int)m.size(1), (int)ctx->saved_data["dtype"].toInt(), m.data_ptr(), m.stride(0), (const uint8_t *)at_or_null(mask),
@@ -301,6 +311,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t seed, const Offset &offset, c
     same(x, residual, "residual", x.scalar_type());
     TORCH_CHECK(residual.sizes() == x.sizes(), "residual: expected shape ", x.sizes(), ", got ", residual.sizes());
   }
+  no_tangents("dropout", {&x, &residual});
   if (torch::GradMode::is_enabled() && (wanted(x) || wanted(residual))) return DropoutFunction::apply(x, residual_, &c);
   return dropout_run(x, residual, c);
 }
@@ -308,6 +319,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t seed, const Offset &offset, c
 std::tuple<Tensor, Tensor> router_balance(const Tensor &logits, const Tensor &ids, const std::optional<Tensor> &mask) {
   BalanceCall c;
   c.dtype = element_type(logits, "logits");
+  no_tangents("router_balance", {&logits});
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= GSDF_ROUTER_MAX_EXPERTS, "logits: expected [..., e] with 1 to ", GSDF_ROUTER_MAX_EXPERTS,
               " experts, got ", logits.sizes());
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

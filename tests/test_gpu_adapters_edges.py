@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import adapters_ref as ref
 from test_gpu_adapters import make
@@ -128,3 +129,24 @@ def test_lowrank_an_infinity_in_one_rank_stays_there(ad, rows, r, dtype):
     db, = torch.autograd.grad(ad.lowrank_adapt(x, a, b, ids, scales, base), leaves[2:], dy)
     assert not torch.isfinite(db[1, :, 2].float()).any()
     check_alone(want, "db", db, 64 + rows, 2, keep)
+
+
+def test_forward_mode_is_refused(ad):
+    """a dual tensor does not ask for a gradient, and its tangent would be lost without an error"""
+    x, a, b, ids, scales, base, _ = make(30, 16, 12, 4, 2, torch.float32)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: ad.lowrank_adapt(dual(x), a, b, ids, scales, base), lambda: ad.lowrank_adapt(x, dual(a), b, ids, scales, base),
+                             lambda: ad.lowrank_adapt(x, a, dual(b), ids, scales, base), lambda: ad.lowrank_adapt(x, a, b, ids, dual(scales), base),
+                             lambda: ad.lowrank_adapt(x, a, b, ids, scales, dual(base)), lambda: ad.lowrank_adapt_(dual(base.clone()), x, a, b, ids, scales),
+                             lambda: ad.lowrank_adapt_(base.clone(), dual(x), a, b, ids, scales), lambda: ad.dropout(dual(x), 0.5, 1),
+                             lambda: ad.dropout(x, 0.5, 1, residual=dual(x)), lambda: ad.router_balance(dual(x), ids)):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call()
+        leaf = x.clone().requires_grad_(True)
+        for y in (ad.lowrank_adapt(leaf, a, b, ids, scales, base), ad.dropout(leaf, 0.5, 1), ad.router_balance(leaf, ids)[0]):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, dual(y.detach()), retain_graph=True)
+            torch.autograd.grad(y, leaf, y.detach())      # nobody is dual: as ever
