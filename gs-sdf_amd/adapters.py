@@ -8,8 +8,8 @@ the router that chooses them (include/gsdf_hip.h: L1-L3).  No reference counterp
 
 Elements are fp32, fp16 or bf16 (one type per call), sums are held in 32 bits and a result is rounded once.  Rows may be strided (a slice of a wider
 buffer is read in place); any other layout is copied first.  Every call runs on the current stream of its tensors' device, allocates its
-workspace from torch's caching allocator and can be captured into a graph; nothing synchronises.  Derivatives are those of a backward pass: an input with a
-forward-mode tangent is refused.  As with every operator of torch, a backward pass is captured
+workspace from torch's caching allocator and can be captured into a graph; nothing synchronises.  Derivatives are those of one backward pass: a second one
+through a gradient raises (through base and residual, which are added as they are, it goes on), an input with a forward-mode tangent is refused.  As with every operator of torch, a backward pass is captured
 only while no eager graph of the same leaves lives: torch would wait for that graph's stream, which ends the capture and may end the process.
 """
 import importlib.util

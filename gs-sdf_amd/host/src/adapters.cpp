@@ -64,18 +64,13 @@ void *at_or_null(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr;
 Tensor bytes(const Tensor &ref, size_t n) { return torch::empty({(int64_t)n}, ref.options().dtype(torch::kUInt8).requires_grad(false)); }
 Tensor plain(const Tensor &ref, at::IntArrayRef shape) { return torch::empty(shape, ref.options().requires_grad(false)); }
 
-// a gradient that somebody wants to differentiate again (create_graph): that raises, instead of taking it for a constant
-variable_list once(const char *name, variable_list grads) {
-  if (!torch::GradMode::is_enabled()) return grads;
-  variable_list some;
-  for (const Tensor &g : grads)
-    if (g.defined()) some.push_back(g.detach().requires_grad_(true));
-  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + ": differentiable once only", (int64_t)some.size());
-  some = (*error)(std::move(some));
-  size_t k = 0;
-  for (Tensor &g : grads)
-    if (g.defined()) g = some[k++];
-  return grads;
+// A gradient that somebody wants to differentiate again (create_graph): that raises, instead of taking it for a constant.  `of`: what it depends on, so that the
+// error lies on the way to every leaf behind it, also where torch.autograd.grad asks for that leaf alone.
+Tensor once(const char *name, const Tensor &grad, variable_list of) {
+  if (!torch::GradMode::is_enabled() || !grad.defined()) return grad;
+  of.insert(of.begin(), grad.detach());
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + ": differentiable once only", (int64_t)of.size());
+  return (*error)(std::move(of))[0];
 }
 
 // ---- L1 -------------------------------------------------------------------------------------------------------------------------------------
@@ -110,8 +105,7 @@ Tensor lowrank_run(const Tensor &x, const Tensor &a, const Tensor &b, const Lowr
 }
 
 struct LowrankFunction : public torch::autograd::Function<LowrankFunction> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &a, const Tensor &b, const std::optional<Tensor> &base, const LowrankCall *c) {
-    const Tensor x = matrix(x_);
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &a, const Tensor &b, const std::optional<Tensor> &base, const LowrankCall *c) {
     Tensor y = plain(x, {x.size(0), b.size(1)});
     const Tensor save = lowrank_run(x, a, b, *c, base.value_or(Tensor()), y, true);
     ctx->save_for_backward({x, a, b, c->ids, c->scales, c->word, save});
@@ -139,7 +133,7 @@ struct LowrankFunction : public torch::autograd::Function<LowrankFunction> {
       check(gsdf_lowrank_bwd(&args, g.data_ptr(), g.stride(0), save.data_ptr(), at_or_null(dx), need_x ? dx.stride(0) : 0, at_or_null(da), at_or_null(db),
                              ws.data_ptr(), stream_of(x)), "lowrank_adapt's backward pass");
     }
-    return once("lowrank_adapt", {dx, da, db, need_base ? dy : Tensor(), Tensor()});
+    return {once("lowrank_adapt", dx, {dy, a, b}), once("lowrank_adapt", da, {dy, x, b}), once("lowrank_adapt", db, {dy, x, a}), need_base ? dy : Tensor(), Tensor()};
   }
 };
 
@@ -224,7 +218,8 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
     no_tangents("dropout's backward pass", {&dy});
     const DropoutCall c{ctx->get_saved_variables()[0], (int)ctx->saved_data["dtype"].toInt(), ctx->saved_data["p"].toDouble(),
                         (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()};
-    return once("dropout", {ctx->needs_input_grad(0) ? dropout_run(dy, Tensor(), c) : Tensor(), ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? dy : Tensor(), Tensor()});
+    return {ctx->needs_input_grad(0) ? once("dropout", dropout_run(dy, Tensor(), c), {dy}) : Tensor(),
+            ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? dy : Tensor(), Tensor()};
   }
 };
 
@@ -247,8 +242,7 @@ std::tuple<Tensor, Tensor, Tensor> balance_run(const Tensor &m, const BalanceCal
   return {loss, counts, pull};
 }
 struct BalanceFunction : public torch::autograd::Function<BalanceFunction> {
-  static variable_list forward(AutogradContext *ctx, const Tensor &logits, const BalanceCall *c) {
-    const Tensor m = matrix(logits);
+  static variable_list forward(AutogradContext *ctx, const Tensor &m, const BalanceCall *c) {
     auto [loss, counts, pull] = balance_run(m, *c);
     ctx->save_for_backward({m, c->mask, pull});
     ctx->saved_data["dtype"] = (int64_t)c->dtype;
@@ -264,7 +258,7 @@ struct BalanceFunction : public torch::autograd::Function<BalanceFunction> {
     const Tensor v = grads[0].to(torch::kFloat32).contiguous(), out = plain(m, {m.size(0), m.size(1)});
     check(gsdf_router_balance_bwd(m.size(0), (int)m.size(1), (int)ctx->saved_data["dtype"].toInt(), m.data_ptr(), m.stride(0), (const uint8_t *)at_or_null(mask),
                                   pull.data_ptr<float>(), v.data_ptr<float>(), out.data_ptr(), stream_of(m)), "router_balance's backward pass");
-    return once("router_balance", {out, Tensor()});
+    return {once("router_balance", out, {grads[0], m}), Tensor()};
   }
 };
 
@@ -277,9 +271,9 @@ Tensor lowrank_adapt(const Tensor &x, const Tensor &a_, const Tensor &b_, const 
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = b.size(1);
   if (torch::GradMode::is_enabled() && (wanted(x) || wanted(a) || wanted(b) || wanted(base))) {
-    if (x.dim() == 2) return LowrankFunction::apply(x, a, b, base_, &c);
-    const int64_t rows = c.ids.numel();
-    return LowrankFunction::apply(x.reshape({rows, x.size(-1)}), a, b, base_ ? std::optional<Tensor>(base.reshape({rows, b.size(1)})) : base_, &c).view(shape);
+    const Tensor m = matrix(x);      // (out here: what the node saves keeps its history)
+    if (x.dim() == 2) return LowrankFunction::apply(m, a, b, base_, &c);
+    return LowrankFunction::apply(m, a, b, base_ ? std::optional<Tensor>(matrix(base)) : base_, &c).view(shape);
   }
   const Tensor m = matrix(x), y = plain(x, shape);
   lowrank_run(m, a, b, c, base, y.dim() == 2 ? y : y.view({m.size(0), b.size(1)}), false);
@@ -336,9 +330,7 @@ std::tuple<Tensor, Tensor> router_balance(const Tensor &logits, const Tensor &id
     c.mask = whole(*mask);
   }
   if (torch::GradMode::is_enabled() && wanted(logits)) {
-    int64_t rows = 1;
-    for (const int64_t n : lead) rows *= n;
-    const variable_list r = BalanceFunction::apply(logits.dim() == 2 ? logits : logits.reshape({rows, logits.size(-1)}), &c);
+    const variable_list r = BalanceFunction::apply(matrix(logits), &c);
     return {r[0], r[1]};
   }
   auto [loss, counts, pull] = balance_run(matrix(logits), c);

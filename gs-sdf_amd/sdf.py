@@ -450,7 +450,8 @@ class TCNNNetwork:
 
     def forward(self, x, adapters=None, ids=None):
         """`adapters`, `ids` (not in the reference's interface): low-rank adapters (adapters.LowRankAdapters, n_in -> n_out of this network) beside the
-        shared network, row i takes adapter ids[i] (outside [0, n_adapters): none) — one decoder for the points of many maps."""
+        shared network, row i takes adapter ids[i] (outside [0, n_adapters): none) — one decoder for the points of many maps.  The adapters' gradients are
+        differentiable once: a loss on the gradient of what comes out of them raises."""
         if x.dim() != 2 or x.shape[1] != self.dims[0]:
             raise RuntimeError(f"TCNNNetwork.forward: expected [B,{self.dims[0]}]")
         if (adapters is None) != (ids is None):

@@ -150,3 +150,36 @@ def test_forward_mode_is_refused(ad):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, dual(y.detach()), retain_graph=True)
             torch.autograd.grad(y, leaf, y.detach())      # nobody is dual: as ever
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_second_derivatives_raise_and_are_not_taken_for_nothing(ad, strided):
+    """by backward() and by grad(), which asks for some leaves alone: beside a term of its own a missing one would go unseen"""
+    x, a, b, ids, scales, base, _ = make(300, 16, 12, 4, 2, torch.float32)
+    x = x.t().contiguous().t() if strided else x
+    leaf = lambda t: t.clone().requires_grad_(True)  # noqa: E731
+    for call, leaves in ((lambda t, u, v: ad.lowrank_adapt(t, u, v, ids, scales, base), [leaf(x), leaf(a), leaf(b)]),
+                         (lambda t, u, v: ad.lowrank_adapt(t.view(30, 10, 16), u, v, ids.view(30, 10), scales), [leaf(x).contiguous().detach().requires_grad_(True), leaf(a), leaf(b)]),
+                         (lambda t: ad.dropout(t, 0.5, 1), [leaf(x)]), (lambda t: ad.router_balance(t, ids)[0], [leaf(x)])):
+        for i in range(len(leaves)):      # the gradient of one factor
+            first, = torch.autograd.grad((call(*leaves) ** 2).sum(), leaves[i], create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                first.sum().backward(retain_graph=True)
+            for other in leaves:
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(first.sum() + (other ** 2).sum(), other, retain_graph=True)
+    x, a, b = [t.detach() for t in (x, a, b)]
+    t = leaf(x)
+    first, = torch.autograd.grad(ad.lowrank_adapt(t, a, b, ids).sum(), t, create_graph=True)      # a constant: there is nothing to refuse
+    assert torch.equal(torch.autograd.grad((t ** 2).sum() + first.sum(), t)[0], 2 * t)
+
+
+def test_what_is_added_stays_differentiable(ad):
+    """base and residual go into the sum as they are, and so do derivatives of every order"""
+    x, a, b, ids, scales, _, _ = make(300, 16, 16, 4, 2, torch.float32)
+    z = torch.randn(300, 16, device="cuda", requires_grad=True)
+    for call in (lambda t: ad.lowrank_adapt(x, a, b, ids, scales, t), lambda t: ad.dropout(x, 0.5, 1, residual=t)):
+        y = call(z ** 3)
+        first, = torch.autograd.grad((y ** 2).sum(), z, create_graph=True)
+        assert torch.allclose(first, 6 * y * z ** 2)
+        assert torch.allclose(torch.autograd.grad(first.sum(), z)[0], 18 * z ** 4 + 12 * y * z, rtol=1e-4, atol=1e-4)
