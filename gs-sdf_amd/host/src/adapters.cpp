@@ -108,6 +108,7 @@ struct LowrankFunction : public torch::autograd::Function<LowrankFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &a, const Tensor &b, const std::optional<Tensor> &base, const LowrankCall *c) {
     Tensor y = plain(x, {x.size(0), b.size(1)});
     const Tensor save = lowrank_run(x, a, b, *c, base.value_or(Tensor()), y, true);
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, a, b, c->ids, c->scales, c->word, save});
     ctx->saved_data["dtype"] = (int64_t)c->dtype;
     ctx->saved_data["p"] = c->p;
@@ -204,6 +205,7 @@ Tensor dropout_run(const Tensor &x, const Tensor &residual, const DropoutCall &c
 }
 struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &residual, const DropoutCall *c) {
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({c->word});
     ctx->saved_data["dtype"] = (int64_t)c->dtype;
     ctx->saved_data["p"] = c->p;
@@ -247,6 +249,7 @@ struct BalanceFunction : public torch::autograd::Function<BalanceFunction> {
     ctx->save_for_backward({m, c->mask, pull});
     ctx->saved_data["dtype"] = (int64_t)c->dtype;
     ctx->mark_non_differentiable({counts});
+    ctx->set_materialize_grads(false);      // (of the counts neither: zeros that nobody reads)
     return {loss, counts};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {

@@ -152,6 +152,26 @@ def test_forward_mode_is_refused(ad):
             torch.autograd.grad(y, leaf, y.detach())      # nobody is dual: as ever
 
 
+class Cut(torch.autograd.Function):
+    """hands its input on and no gradient back"""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def test_no_gradient_upstream_is_no_gradient(ad):
+    x, a, b, ids, scales, base, _ = make(300, 16, 12, 4, 2, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, a, b, base)]
+    for y, of in ((ad.lowrank_adapt(x, a, b, ids, scales, base), leaves), (ad.dropout(x, 0.5, 1), [x]), (ad.dropout(x, 0.5, 1, residual=x * 2), [x]),
+                  (ad.router_balance(x, ids)[0], [x])):
+        assert all(g is None for g in torch.autograd.grad(Cut.apply(y).sum(), of, allow_unused=True))
+
+
 @pytest.mark.parametrize("strided", [False, True])
 def test_second_derivatives_raise_and_are_not_taken_for_nothing(ad, strided):
     """by backward() and by grad(), which asks for some leaves alone: beside a term of its own a missing one would go unseen"""
