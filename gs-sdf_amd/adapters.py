@@ -51,7 +51,7 @@ def lowrank_adapt(x, a, b, ids, scales=None, base=None, p=0.0, seed=0, offset=0)
 
 def lowrank_adapt_(y, x, a, b, ids, scales=None):
     """In place, for serving: y += s_g B_g A_g x in every row that has an adapter; the other rows are not touched.  y [..., n] has neighbouring elements in a row
-    (a slice of a wider buffer is fine) and shares no memory with x.  No gradients."""
+    (a slice of a wider buffer is fine) and shares no memory with what the call reads.  No gradients."""
     (_mod or _ops()).lowrank_adapt_(y, x, a, b, ids, scales)
     return y
 

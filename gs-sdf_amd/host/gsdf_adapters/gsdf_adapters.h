@@ -23,7 +23,7 @@ struct Offset {
 torch::Tensor lowrank_adapt(const torch::Tensor &x, const torch::Tensor &a, const torch::Tensor &b, const torch::Tensor &ids,
                             const std::optional<torch::Tensor> &scales = std::nullopt, const std::optional<torch::Tensor> &base = std::nullopt, double p = 0.0,
                             uint64_t seed = 0, const Offset &offset = {});
-// y += s_g B_g A_g x in place, rows without an adapter untouched; y and x share no memory (else: error); no gradients
+// y += s_g B_g A_g x in place, rows without an adapter untouched; y shares no memory with what the call reads (else: error); no gradients
 void lowrank_adapt_(const torch::Tensor &y, const torch::Tensor &x, const torch::Tensor &a, const torch::Tensor &b, const torch::Tensor &ids,
                     const std::optional<torch::Tensor> &scales = std::nullopt);
 // [residual +] x with elements dropped at probability round(65536 p) / 65536, the others multiplied by 1 / (1 - that)

@@ -175,17 +175,19 @@ LowrankCall lowrank_check(const Tensor &x, Tensor &a, Tensor &b, const Tensor &i
   return c;
 }
 
-// two matrices of one width of element in the same memory: apart, or columns of one buffer that do not meet
-void share_nothing(const Tensor &y, const Tensor &x) {
-  if (y.numel() == 0 || x.numel() == 0) return;
-  const int64_t rows = y.size(0), es = (int64_t)y.element_size(), n = y.size(1) * es, k = x.size(1) * es, stride = y.stride(0) * es;
-  const char *py = (const char *)y.data_ptr(), *px = (const char *)x.data_ptr();
-  if (py + (rows - 1) * stride + n <= px || px + (rows - 1) * x.stride(0) * es + k <= py) return;
-  if (rows > 1 && x.stride(0) == y.stride(0)) {
-    const int64_t by = ((px - py) % stride + stride) % stride;
+// y, written in place, and something the call reads: apart, or columns of one buffer that do not meet (t's rows y's stride apart, or one row between two of y's)
+void share_nothing(const Tensor &y, const Tensor &t, const char *name) {
+  if (y.numel() == 0 || !t.defined() || t.numel() == 0) return;
+  const int64_t es = (int64_t)y.element_size(), et = (int64_t)t.element_size(), rows = y.size(0), n = y.size(1) * es, stride = y.stride(0) * es;
+  const bool matrix = t.dim() == 2;      // (anything else is contiguous)
+  const int64_t rows_t = matrix ? t.size(0) : 1, k = (matrix ? t.size(1) : t.numel()) * et, stride_t = matrix ? t.stride(0) * et : 0;
+  const char *py = (const char *)y.data_ptr(), *pt = (const char *)t.data_ptr();
+  if (py + (rows - 1) * stride + n <= pt || pt + (rows_t - 1) * stride_t + k <= py) return;
+  if (rows > 1 && (rows_t == 1 || stride_t == stride)) {
+    const int64_t by = ((pt - py) % stride + stride) % stride;
     if (by >= n && by + k <= stride) return;
   }
-  TORCH_CHECK(false, "lowrank_adapt_: y and x share memory");
+  TORCH_CHECK(false, "lowrank_adapt_: y and ", name, " share memory");
 }
 
 // ---- L2 -------------------------------------------------------------------------------------------------------------------------------------
@@ -287,11 +289,16 @@ void lowrank_adapt_(const Tensor &y, const Tensor &x, const Tensor &a_, const Te
   Tensor a = a_, b = b_;
   const LowrankCall c = lowrank_check(x, a, b, ids, scales, y, 0.0, 0, {});
   TORCH_CHECK(!(torch::GradMode::is_enabled() && (wanted(y) || wanted(x) || wanted(a) || wanted(b))), "lowrank_adapt_: no gradients in place; use lowrank_adapt");
+  TORCH_CHECK(!y.is_inference() || c10::InferenceMode::is_enabled(), "lowrank_adapt_: y is an inference tensor, outside inference mode");
   const Tensor out = y.dim() == 2 ? y : y.view({c.ids.numel(), b.size(1)});
   TORCH_CHECK(out.stride(1) == 1 || out.size(1) == 1, "lowrank_adapt_: the elements of a row of y have to be neighbours");
   TORCH_CHECK(out.size(0) <= 1 || out.stride(0) >= out.size(1), "lowrank_adapt_: the rows of y overlap");
   const Tensor m = matrix(x);
-  share_nothing(out, m);
+  share_nothing(out, m, "x");
+  share_nothing(out, a, "a");
+  share_nothing(out, b, "b");
+  share_nothing(out, c.ids, "ids");
+  share_nothing(out, c.scales, "scales");
   lowrank_run(m, a, b, c, out, out, false);
   y.unsafeGetTensorImpl()->bump_version();
 }

@@ -203,3 +203,33 @@ def test_what_is_added_stays_differentiable(ad):
         first, = torch.autograd.grad((y ** 2).sum(), z, create_graph=True)
         assert torch.allclose(first, 6 * y * z ** 2)
         assert torch.allclose(torch.autograd.grad(first.sum(), z)[0], 18 * z ** 4 + 12 * y * z, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+def test_lowrank_in_place_refuses_before_it_writes(ad, rows):
+    x, a, b, ids, scales, base, _ = make(rows, 40, 24, 8, 3, torch.float32, 0.1)
+    with torch.inference_mode():
+        y = base.clone()
+        ad.lowrank_adapt_(y, x, a, b, ids, scales)      # in inference mode: as torch's own operators in place
+        y.copy_(base)
+    with pytest.raises(RuntimeError, match="inference"):
+        ad.lowrank_adapt_(y, x, a, b, ids, scales)
+    assert torch.equal(y, base)
+    big = torch.zeros(max(rows * 24, a.numel(), b.numel()) + 64, device="cuda")
+    y = big[16:16 + rows * 24].view(rows, 24)
+    for name, t in (("a", a), ("b", b), ("scales", scales)):
+        inside = big[20:20 + t.numel()].view(t.shape)
+        inside.copy_(t)
+        held = big.clone()
+        with pytest.raises(RuntimeError, match="share memory"):
+            ad.lowrank_adapt_(y, x, inside if name == "a" else a, inside if name == "b" else b, ids, inside if name == "scales" else scales)
+        assert torch.equal(big, held)
+    inside = big.view(torch.int32)[20:20 + rows]
+    inside.copy_(ids)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ad.lowrank_adapt_(y, x, a, b, inside, scales)
+    # weights between the rows of a strided y share nothing with it
+    wide = torch.zeros(rows, 40, device="cuda")
+    wide[0, 30:33] = scales
+    wide[:, :24] = base
+    assert torch.equal(ad.lowrank_adapt_(wide[:, :24], x, a, b, ids, wide[0, 30:33]), ad.lowrank_adapt(x, a, b, ids, scales, base))
