@@ -30,9 +30,11 @@ void same(const Tensor &ref, const Tensor &t, const char *name, torch::ScalarTyp
   same_device(ref, t, name);
   TORCH_CHECK(t.scalar_type() == type, name, ": expected ", type, " elements, got ", t.scalar_type());
 }
+// the tensor's memory holds what the tensor says (a lazily negated view, as conj().imag is one, holds the opposite)
+Tensor plainly(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
 // a [rows, width] matrix whose rows are neighbours' elements: a view where the layout allows it
 Tensor matrix(const Tensor &t) {
-  Tensor m = t;
+  Tensor m = plainly(t);
   if (m.dim() != 2) {
     const int64_t width = m.dim() ? m.size(-1) : 1;
     int64_t rows = 1;
@@ -41,7 +43,10 @@ Tensor matrix(const Tensor &t) {
   }
   return m.stride(1) == 1 || m.size(1) == 1 ? m : m.contiguous();
 }
-Tensor whole(const Tensor &t) { return t.is_contiguous() ? t : t.contiguous(); }
+Tensor whole(const Tensor &t) {
+  const Tensor p = plainly(t);
+  return p.is_contiguous() ? p : p.contiguous();
+}
 Tensor index(const Tensor &ref, const Tensor &t, const char *name) {
   same_device(ref, t, name);
   TORCH_CHECK(t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64, name, ": expected int32 or int64, got ", t.scalar_type());
@@ -260,7 +265,7 @@ struct BalanceFunction : public torch::autograd::Function<BalanceFunction> {
     if (!grads[0].defined()) return variable_list(2);
     no_tangents("router_balance's backward pass", {&grads[0]});
     const c10::DeviceGuard guard(m.device());
-    const Tensor v = grads[0].to(torch::kFloat32).contiguous(), out = plain(m, {m.size(0), m.size(1)});
+    const Tensor v = whole(grads[0].to(torch::kFloat32)), out = plain(m, {m.size(0), m.size(1)});
     check(gsdf_router_balance_bwd(m.size(0), (int)m.size(1), (int)ctx->saved_data["dtype"].toInt(), m.data_ptr(), m.stride(0), (const uint8_t *)at_or_null(mask),
                                   pull.data_ptr<float>(), v.data_ptr<float>(), out.data_ptr(), stream_of(m)), "router_balance's backward pass");
     return {once("router_balance", out, {grads[0], m}), Tensor()};
@@ -289,6 +294,7 @@ void lowrank_adapt_(const Tensor &y, const Tensor &x, const Tensor &a_, const Te
   Tensor a = a_, b = b_;
   const LowrankCall c = lowrank_check(x, a, b, ids, scales, y, 0.0, 0, {});
   TORCH_CHECK(!(torch::GradMode::is_enabled() && (wanted(y) || wanted(x) || wanted(a) || wanted(b))), "lowrank_adapt_: no gradients in place; use lowrank_adapt");
+  TORCH_CHECK(!y.is_neg(), "lowrank_adapt_: y is a lazily negated view");
   TORCH_CHECK(!y.is_inference() || c10::InferenceMode::is_enabled(), "lowrank_adapt_: y is an inference tensor, outside inference mode");
   const Tensor out = y.dim() == 2 ? y : y.view({c.ids.numel(), b.size(1)});
   TORCH_CHECK(out.stride(1) == 1 || out.size(1) == 1, "lowrank_adapt_: the elements of a row of y have to be neighbours");

@@ -205,6 +205,24 @@ def test_what_is_added_stays_differentiable(ad):
         assert torch.allclose(torch.autograd.grad(first.sum(), z)[0], 18 * z ** 4 + 12 * y * z, rtol=1e-4, atol=1e-4)
 
 
+def test_lazily_negated_tensors(ad):
+    x, a, b, ids, scales, base, dy = make(300, 16, 16, 4, 2, torch.float32)
+    neg = torch._neg_view
+    assert neg(x).is_neg()
+    want = ad.lowrank_adapt(-x, a, -b, ids, -scales, -base)
+    assert torch.equal(ad.lowrank_adapt(neg(x), a, neg(b), ids, neg(scales), neg(base)), want)
+    assert torch.equal(ad.lowrank_adapt(x, neg(a), b, ids), ad.lowrank_adapt(x, -a, b, ids))
+    assert torch.equal(ad.dropout(neg(x), 0.5, 1, residual=neg(dy)), ad.dropout(-x, 0.5, 1, residual=-dy))
+    assert torch.equal(ad.router_balance(neg(x), ids)[0], ad.router_balance(-x, ids)[0])
+    leaf = x.clone().requires_grad_(True)
+    got, = torch.autograd.grad(ad.lowrank_adapt(neg(leaf), a, b, ids), leaf, neg(dy))
+    assert torch.equal(got, torch.autograd.grad(ad.lowrank_adapt(-leaf, a, b, ids), leaf, -dy)[0])
+    out = base.clone()
+    with pytest.raises(RuntimeError, match="negat"):
+        ad.lowrank_adapt_(neg(out), x, a, b, ids)
+    assert torch.equal(out, base)
+
+
 @pytest.mark.parametrize("rows", [6, 300])
 def test_lowrank_in_place_refuses_before_it_writes(ad, rows):
     x, a, b, ids, scales, base, _ = make(rows, 40, 24, 8, 3, torch.float32, 0.1)
