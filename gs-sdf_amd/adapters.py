@@ -59,14 +59,18 @@ def lowrank_adapt_(y, x, a, b, ids, scales=None):
 class LowRankAdapters:
     """Adapters for a shared network (sdf.TCNNNetwork.forward takes them): leaves `a_` [n_adapters, rank, n_in] (uniform, bound 1 / sqrt(n_in)) and `b_`
     [n_adapters, n_out, rank] (zeros: a new adapter changes nothing), scale alpha / rank.  p > 0: dropout on their input in every call that makes gradients;
-    its masks go by `seed` and `calls_`, which counts such calls.  `calls_` is a host number: a captured call replays one mask, so give
-    `offset` (a device word that the program counts up) there."""
+    its masks go by `seed` and `calls_`, which counts such calls: both belong into a checkpoint beside the leaves.  Without a `seed` every bank has another, out of
+    torch's default generator (torch.manual_seed makes them again; processes that train one bank give one seed), since two banks of one seed drop the same elements.  `calls_` is a host number: a
+    captured call replays one mask and a call that is made again for its gradients (activation checkpoints) takes another, so give `offset` (a number of the program's own, or a
+    device word that it counts up) there."""
 
-    def __init__(self, n_adapters, n_in, n_out, rank, alpha=None, p=0.0, dtype=torch.float32, device="cuda", seed=0):
+    def __init__(self, n_adapters, n_in, n_out, rank, alpha=None, p=0.0, dtype=torch.float32, device="cuda", seed=None):
         if not (1 <= rank <= MAX_RANK and 1 <= n_adapters <= MAX_ADAPTERS):
             raise RuntimeError(f"LowRankAdapters: rank {rank} or {n_adapters} adapters out of range")
         if not 0.0 <= float(p) <= 1.0:
             raise RuntimeError(f"p: expected a probability in [0, 1], got {p}")
+        if seed is None:
+            seed = int(torch.randint(0, 1 << 62, (), device="cpu"))
         g = torch.Generator(device="cpu").manual_seed(seed)
         self.a_ = ((torch.rand(n_adapters, rank, n_in, generator=g) * 2 - 1) / math.sqrt(n_in)).to(dtype).to(device).requires_grad_(True)
         self.b_ = torch.zeros(n_adapters, n_out, rank, dtype=dtype, device=device).requires_grad_(True)

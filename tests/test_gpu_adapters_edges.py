@@ -251,3 +251,22 @@ def test_lowrank_in_place_refuses_before_it_writes(ad, rows):
     wide[0, 30:33] = scales
     wide[:, :24] = base
     assert torch.equal(ad.lowrank_adapt_(wide[:, :24], x, a, b, ids, wide[0, 30:33]), ad.lowrank_adapt(x, a, b, ids, scales, base))
+
+
+def test_banks_made_without_a_seed_differ(ad):
+    """two layers' banks drop different elements and begin with different weights; torch's own seed makes them again"""
+    x = torch.ones(200, 64, device="cuda", requires_grad=True)
+    ids = torch.zeros(200, dtype=torch.int32, device="cuda")
+
+    def mask(bank):      # through weights that change nothing
+        with torch.no_grad():
+            bank.a_[0].copy_(torch.eye(64)), bank.b_[0].copy_(torch.eye(64))
+        return bank(x, ids).detach() == 0
+    torch.manual_seed(5)
+    banks = [ad.LowRankAdapters(2, 64, 64, 64, p=0.5) for _ in range(2)]
+    assert banks[0].seed != banks[1].seed and not torch.equal(banks[0].a_, banks[1].a_)
+    torch.manual_seed(5)
+    again = ad.LowRankAdapters(2, 64, 64, 64, p=0.5)
+    assert again.seed == banks[0].seed and torch.equal(again.a_, banks[0].a_)
+    assert not torch.equal(mask(banks[0]), mask(banks[1]))
+    assert torch.equal(ad.LowRankAdapters(2, 64, 64, 64, seed=3).a_, ad.LowRankAdapters(2, 64, 64, 64, seed=3).a_)
