@@ -58,7 +58,8 @@ def lowrank_adapt_(y, x, a, b, ids, scales=None):
 
 class LowRankAdapters:
     """Adapters for a shared network (sdf.TCNNNetwork.forward takes them): leaves `a_` [n_adapters, rank, n_in] (uniform, bound 1 / sqrt(n_in)) and `b_`
-    [n_adapters, n_out, rank] (zeros: a new adapter changes nothing), scale alpha / rank.  p > 0: dropout on their input in every call that makes gradients;
+    [n_adapters, n_out, rank] (zeros: a new adapter changes nothing), scale alpha / rank.  p > 0: dropout on their input in every call that makes gradients, until eval() (a normal taken for an
+    answer makes gradients too; train() turns it on again);
     its masks go by `seed` and `calls_`, which counts such calls: both belong into a checkpoint beside the leaves.  Without a `seed` every bank has another, out of
     torch's default generator (torch.manual_seed makes them again; processes that train one bank give one seed), since two banks of one seed drop the same elements.  `calls_` is a host number: a
     captured call replays one mask and a call that is made again for its gradients (activation checkpoints) takes another, so give `offset` (a number of the program's own, or a
@@ -75,11 +76,18 @@ class LowRankAdapters:
         self.a_ = ((torch.rand(n_adapters, rank, n_in, generator=g) * 2 - 1) / math.sqrt(n_in)).to(dtype).to(device).requires_grad_(True)
         self.b_ = torch.zeros(n_adapters, n_out, rank, dtype=dtype, device=device).requires_grad_(True)
         self.scales = torch.full((n_adapters,), float(rank if alpha is None else alpha) / rank, dtype=torch.float32, device=device)
-        self.p, self.seed, self.calls_ = float(p), int(seed), 0
+        self.p, self.seed, self.calls_, self.training = float(p), int(seed), 0, True
+
+    def train(self, mode=True):
+        self.training = bool(mode)
+        return self
+
+    def eval(self):
+        return self.train(False)
 
     def forward(self, x, ids, base=None, offset=None):
-        training = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.a_, self.b_, base))
-        p = self.p if training else 0.0
+        gradients = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.a_, self.b_, base))
+        p = self.p if self.training and gradients else 0.0
         if offset is None:
             offset = self.calls_
             self.calls_ += p > 0

@@ -270,3 +270,19 @@ def test_banks_made_without_a_seed_differ(ad):
     assert again.seed == banks[0].seed and torch.equal(again.a_, banks[0].a_)
     assert not torch.equal(mask(banks[0]), mask(banks[1]))
     assert torch.equal(ad.LowRankAdapters(2, 64, 64, 64, seed=3).a_, ad.LowRankAdapters(2, 64, 64, 64, seed=3).a_)
+
+
+def test_a_bank_that_answers_drops_nothing_even_with_gradients(ad):
+    """a normal at inference is a gradient: eval() takes the dropout out and holds the counter"""
+    bank = ad.LowRankAdapters(3, 32, 8, 4, p=0.5, seed=7)
+    with torch.no_grad():
+        bank.b_.normal_()
+    x = torch.randn(100, 32, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 3, (100,), device="cuda", dtype=torch.int32)
+    assert bank.training and bank.eval() is bank and not bank.training
+    y = bank(x, ids)
+    assert torch.equal(y, ad.lowrank_adapt(x, bank.a_, bank.b_, ids, bank.scales)) and bank.calls_ == 0
+    assert bank.train() is bank and bank.training
+    assert torch.equal(bank(x, ids), ad.lowrank_adapt(x, bank.a_, bank.b_, ids, bank.scales, p=0.5, seed=7, offset=0)) and bank.calls_ == 1
+    bank.train(False)
+    assert torch.equal(bank(x, ids), y) and bank.calls_ == 1
