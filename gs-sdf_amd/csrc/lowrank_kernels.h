@@ -1000,8 +1000,11 @@ __global__ void __launch_bounds__(1024) lowrank_row_kernel(RowArgs q) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------------
-// Without gradients, few rows take no plan, which costs 10 us before the first product: where an adapter has hardly more than four of them, and where reading
-// the weights again for every row is no more than this (bf16, 4096 -> 4096: rank 16, 192 rows 12 us against 18, 64 rows of rank 128 16 to 24 against 33).
+// Without gradients, few rows take no plan, which costs 10 us and the layout of every adapter's A before the first product, but read the weights again for every row.
+// Up to 64 rows always (bf16, 4096 -> 4096, rank 64: 13 to 15 us against 23); up to 512, or four an adapter, while what the rows read is no more than 32 MB and
+// twice the weights of all adapters (a choice between rows that are all of one adapter, and stay in a cache, and rows that are of all).  bf16, 4096 -> 4096: 8 adapters of rank 16, 128 rows 11 us
+// against 17; 1024 of rank 64, 2048 rows 191 us against 247 where they are of one adapter and 361 against 413 where they are of all, 4096 rows 352 against 253 and 679 against 445; 128 of
+// rank 64, 256 rows 28 and 47 against 42 and 52, 512 rows 49 and 80 against 43 and 55.  64 -> 4096, 1000 of rank 16, 800 rows: 20 and 29 against 33 and 45.
 static constexpr int64_t LR_FEW_BYTES = 32 << 20;
 static constexpr int64_t LR_FEW_ROWS = 64;
 // bytes of A that may be read to make every row's h again in each of its workgroups, for a launch less
@@ -1090,7 +1093,9 @@ void lowrank_fwd(const Lowrank &q, const void *base, int64_t base_stride, void *
   const gsdf_lowrank_args &a = q.a;
   const Ids ids = {a.ids, a.ids_64, a.n_adapters};
   const int64_t read = a.rows * a.rank * ((int64_t)a.n_in + a.n_out) * (int64_t)sizeof(T);      // of the adapters' weights, row by row
-  if (!training && (a.rows <= LR_FEW_ROWS || a.rows <= 4 * (int64_t)a.n_adapters || (a.rows <= 8 * LR_FEW_ROWS && read <= LR_FEW_BYTES))) {
+  const int64_t bank = (int64_t)a.n_adapters * q.rp * ((int64_t)a.n_in + a.n_out) * (int64_t)sizeof(T);      // all weights, ranks in whole tiles
+  const int64_t most = 4 * (int64_t)a.n_adapters > 8 * LR_FEW_ROWS ? 4 * (int64_t)a.n_adapters : 8 * LR_FEW_ROWS;
+  if (!training && (a.rows <= LR_FEW_ROWS || (a.rows <= most && read <= LR_FEW_BYTES + 2 * bank))) {
     constexpr int N = 16 / (int)sizeof(T);
     RowArgs r;
     r.ids = ids; r.x = a.x; r.a = a.a; r.b = a.b; r.base = base; r.y = y; r.h = q.h; r.x_stride = a.x_stride; r.base_stride = base_stride; r.y_stride = y_stride;

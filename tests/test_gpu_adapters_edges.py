@@ -131,6 +131,19 @@ def test_lowrank_an_infinity_in_one_rank_stays_there(ad, rows, r, dtype):
     check_alone(want, "db", db, 64 + rows, 2, keep)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [65, 1170, 1200, 1300, 1320, 2119])
+@pytest.mark.parametrize("used", [1, 530])
+def test_lowrank_few_adapters_of_a_large_bank(ad, rows, used, dtype):
+    """on both sides of the border between the path of few rows and the plan, which goes by the bytes of weights that either reads"""
+    x, a, b, ids, scales, base, _ = make(rows, 64, 1000, 64, 530, dtype, 0.1)
+    ids = torch.where(ids < 0, ids, ids % used + (530 - used))
+    want = ref.Lowrank(x, a[530 - used:], b[530 - used:], torch.where(ids < 0, ids, ids - (530 - used)), scales[530 - used:], base)
+    got = ad.lowrank_adapt(x, a, b, ids, scales, base)
+    want.check("y", got, 64 + 64)
+    assert torch.equal(got[ids < 0], base[ids < 0])
+
+
 def test_forward_mode_is_refused(ad):
     """a dual tensor does not ask for a gradient, and its tangent would be lost without an error"""
     x, a, b, ids, scales, base, _ = make(30, 16, 12, 4, 2, torch.float32)
