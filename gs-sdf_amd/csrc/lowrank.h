@@ -10,6 +10,7 @@ static constexpr int LR_RANGE = 48;         // most rows of a range: three matri
 static constexpr int LR_BOTH = 65536;        // rows from which on a wave takes a range through both products
 static constexpr int LR_PLAN_ONE = 16384;    // rows up to which the plan is one launch
 static constexpr int LR_CHUNK = 1024;       // most rows of one sum in `outer`
+static constexpr int LR_OUTER_THREADS = 512;
 static constexpr int LR_CHUNK_FEW = 2048;   // the same where all rows are no more: then no adapter has two, and nothing is left to add up
 
 // ---- the rows in the order of their adapters ----------------------------------------------------------------------------------------------

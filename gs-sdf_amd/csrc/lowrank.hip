@@ -386,9 +386,13 @@ extern "C" int gsdf_lowrank_bwd(const gsdf_lowrank_args *args, const void *dy, i
   GSDF_REQUIRE(ws != nullptr && save != nullptr && (args->rows == 0 || dy != nullptr), "lowrank_bwd: dy, the forward's saved buffer and the workspace are required");
   GSDF_REQUIRE(args->rows <= 1 || (dy_stride >= 0 && (dx == nullptr || dx_stride >= args->n_in)), "lowrank_bwd: row strides %lld, %lld", (long long)dy_stride,
                (long long)dx_stride);
-  GSDF_TIMED("gsdf_lowrank_bwd");
   Lowrank q;
   lowrank_layout(&q, args, const_cast<void *>(save), ws, true);
+  // (only rows that lie on one another are so many and so wide)
+  const int64_t columns = 256 / q.es, outer = (int64_t)q.plan.max_chunks * (ceil_div(args->n_in, columns) + ceil_div(args->n_out, columns));
+  GSDF_REQUIRE((da == nullptr && db == nullptr) || outer * LR_OUTER_THREADS < (1ll << 32), "lowrank_bwd: %lld workgroups for the weights' gradients are more than a launch holds",
+               (long long)outer);
+  GSDF_TIMED("gsdf_lowrank_bwd");
   GSDF_BY_DTYPE(args->dtype, lowrank_bwd<T>(q, dy, dy_stride, dx, dx_stride, da, db, stream));
   GSDF_CHECK_LAUNCH("lowrank_bwd");
   return GSDF_OK;

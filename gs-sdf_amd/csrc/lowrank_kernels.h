@@ -628,7 +628,7 @@ __device__ __forceinline__ u32x4 column_of(const u32x4 (&v)[8], int e) {
   return o;
 }
 template <typename T, int RT, bool RAGGED>      // RAGGED: a width is no multiple of COLS
-__global__ void __launch_bounds__(512) lowrank_outer_kernel(OuterArgs q) {
+__global__ void __launch_bounds__(LR_OUTER_THREADS) lowrank_outer_kernel(OuterArgs q) {
   typedef typename Vec<T>::vec V;
   constexpr int VE = Vec<T>::N, COLS = 16 * VE;      // elements of a lane's piece, columns of a workgroup
   __shared__ f32x4 s_sum[4][VE][64];
@@ -1137,9 +1137,9 @@ void lowrank_bwd(const Lowrank &q, const void *dy, int64_t dy_stride, void *dx, 
     const dim3 grid((unsigned)o.blocks * (unsigned)q.plan.max_chunks, q.rt == 8 ? 2 : 1);
     const bool ragged = a.n_in % COLS != 0 || a.n_out % COLS != 0;
     switch (q.rt) {
-      case 1: ragged ? lowrank_outer_kernel<T, 1, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 1, false><<<grid, 512, 0, stream>>>(o); break;
-      case 2: ragged ? lowrank_outer_kernel<T, 2, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 2, false><<<grid, 512, 0, stream>>>(o); break;
-      default: ragged ? lowrank_outer_kernel<T, 4, true><<<grid, 512, 0, stream>>>(o) : lowrank_outer_kernel<T, 4, false><<<grid, 512, 0, stream>>>(o); break;
+      case 1: ragged ? lowrank_outer_kernel<T, 1, true><<<grid, LR_OUTER_THREADS, 0, stream>>>(o) : lowrank_outer_kernel<T, 1, false><<<grid, LR_OUTER_THREADS, 0, stream>>>(o); break;
+      case 2: ragged ? lowrank_outer_kernel<T, 2, true><<<grid, LR_OUTER_THREADS, 0, stream>>>(o) : lowrank_outer_kernel<T, 2, false><<<grid, LR_OUTER_THREADS, 0, stream>>>(o); break;
+      default: ragged ? lowrank_outer_kernel<T, 4, true><<<grid, LR_OUTER_THREADS, 0, stream>>>(o) : lowrank_outer_kernel<T, 4, false><<<grid, LR_OUTER_THREADS, 0, stream>>>(o); break;
     }
   }
   if (a.rows <= q.plan.chunk_rows) return;      // no adapter has two chunks

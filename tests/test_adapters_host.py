@@ -112,3 +112,12 @@ def test_python_entries_refuse_host_tensors():
         adapters.LowRankAdapters(2, 8, 5, 129, device="cpu")
     with pytest.raises(RuntimeError, match="probability"):
         adapters.LowRankAdapters(2, 8, 5, 4, p=1.5, device="cpu")
+
+
+def test_lowrank_refuses_weight_gradients_behind_a_launch(capi):
+    """rows that are one row again and again make more workgroups of 512 threads than a launch holds (2^32 threads) out of little memory"""
+    L = capi.lib()
+    for bad in (dict(rows=(1 << 28) - 1, n_in=1 << 21, x_stride=0, n_out=8, rank=1, n_adapters=1), dict(rows=1 << 26, n_in=8, n_out=1 << 21, rank=4, n_adapters=1, dtype=2)):
+        args = _args(capi, **bad)
+        assert L.gsdf_lowrank_bwd(C.byref(args), 64, 0, 64, None, 0, 64, 64, 64, None) == -1
+        assert "a launch" in L.gsdf_last_error().decode()
