@@ -13,7 +13,7 @@ while [ $# -gt 0 ]; do
   while [ $# -gt 0 ] && [ "$1" != "--" ]; do FLAGS+=("$1"); shift; done
   [ "${1:-}" = "--" ] && shift
   STEM=$(basename $SRC .hip)
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I$ROOT/include -I$ROOT/gs-sdf_amd/csrc "${FLAGS[@]}" -c $ROOT/gs-sdf_amd/csrc/$SRC -o $OUT/obj/$STEM.o
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -I$ROOT/include -I$ROOT/gs-sdf_amd/csrc "${FLAGS[@]}" -c $ROOT/gs-sdf_amd/csrc/$SRC -o $OUT/obj/$STEM.o
   OBJS=$(echo "$OBJS" | grep -v "/$STEM.o")
   OBJS="$OBJS $OUT/obj/$STEM.o"
 done

@@ -16,6 +16,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "gs-sdf_amd", "csrc")
 NO_CONTRACT = {"projection", "binning", "radix", "occupancy", "marching_cubes", "refine"}      # as the Makefile builds them
 NO_SLP = {"raster_fwd", "raster_bwd"}
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 PAT = re.compile(r"- \.agpr_count:\s+(\d+).*?\.group_segment_fixed_size:\s+(\d+).*?\.max_flat_workgroup_size:\s+(\d+).*?\.name:\s+(\S+).*?"
                  r"\.private_segment_fixed_size:\s+(\d+).*?\.sgpr_count:\s+(\d+).*?\.sgpr_spill_count:\s+(\d+).*?\.vgpr_count:\s+(\d+).*?"
                  r"\.vgpr_spill_count:\s+(\d+)", re.S)
@@ -23,7 +24,7 @@ PAT = re.compile(r"- \.agpr_count:\s+(\d+).*?\.group_segment_fixed_size:\s+(\d+)
 
 def assemble(src, out):
     stem = os.path.basename(src)[:-4]
-    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", f"-I{ROOT}/include", f"-I{CSRC}", "--cuda-device-only", "-S", src, "-o", out]
+    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", *NO_PACKED_FP32, f"-I{ROOT}/include", f"-I{CSRC}", "--cuda-device-only", "-S", src, "-o", out]
     if stem in NO_CONTRACT:
         cmd.insert(4, "-ffp-contract=off")
     if stem in NO_SLP:
@@ -51,7 +52,7 @@ def main(path):
                 waves_cu = min(waves_v * 4, wgs_lds * wg_waves, 32)
                 rows.append((os.path.basename(o)[:-2], dem, vg, int(ag), int(sg), lds, int(priv), int(vgs), int(sgs), wg, waves_v, waves_cu))
     with open(path, "w") as f:
-        f.write("# hipcc --offload-arch=gfx950 -O3, code-object metadata (tools/kernel_resources.py); vgpr = architectural + accumulation registers per lane;\n"
+        f.write("# hipcc --offload-arch=gfx950 -O3 without packed fp32, code-object metadata (tools/kernel_resources.py); vgpr = architectural + accumulation registers per lane;\n"
                 "# waves/SIMD = what the VGPR count allows (<= 8); waves/CU = min of that x 4 SIMDs and the workgroups 160 KB of LDS hold (launch bounds as compiled)\n")
         f.write(f"{'file':16s} {'kernel':56s} {'vgpr':>5s} {'agpr':>5s} {'sgpr':>5s} {'lds B':>7s} {'scratch B':>9s} {'vgpr spills':>11s} {'wg':>5s} {'waves/SIMD':>10s} {'waves/CU':>8s}\n")
         for r in rows:
