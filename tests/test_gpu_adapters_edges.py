@@ -299,3 +299,59 @@ def test_a_bank_that_answers_drops_nothing_even_with_gradients(ad):
     assert torch.equal(bank(x, ids), ad.lowrank_adapt(x, bank.a_, bank.b_, ids, bank.scales, p=0.5, seed=7, offset=0)) and bank.calls_ == 1
     bank.train(False)
     assert torch.equal(bank(x, ids), y) and bank.calls_ == 1
+
+
+@pytest.mark.parametrize("p", [1.0, 65535 / 65536, 1 / 65536])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,k,n,r", [(5, 200, 96, 16), (60, 2048, 1024, 32), (900, 136, 72, 12), (66000, 64, 64, 8)])
+def test_lowrank_masks_at_the_ends_of_p(ad, rows, k, n, r, dtype, p):
+    """everything dropped, all but one element in 65536, that one alone: on the path of few rows, behind the plan, and through both products at once"""
+    x, a, b, ids, scales, base, dy = make(rows, k, n, r, 4, dtype, 0.1)
+    if 0.5 < p < 1:
+        a = a / 256      # the factor of what stays is 65536
+    want = ref.Lowrank(x, a, b, ids, scales, base, dy, p, 21, 22)
+    want.check("y", ad.lowrank_adapt(x, a, b, ids, scales, base, p=p, seed=21, offset=22), k + r)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = ad.lowrank_adapt(x, a, b, ids, scales, base, p=p, seed=21, offset=22)
+    want.check("y", y, k + r)
+    dx, da, db = torch.autograd.grad(y, leaves, dy)
+    f = ref.keep_factor(rows, k, p, 21, 22)
+    assert (dx.cpu()[f == 0] == 0).all()
+    if p == 1.0:
+        assert torch.equal(y, base) and (da == 0).all() and (db == 0).all()
+    if dtype != torch.float16 or p < 0.5 or p == 1.0:      # (65536 times a gradient passes the largest fp16 number)
+        want.check("dx", dx, n + r)
+        want.check("da", da, n + rows)
+        want.check("db", db, k + rows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,cols,p", [(257, 333, 0.3), (64, 64, 0.1), (1, 100003, 0.5), (300, 8, 65535 / 65536), (70, 1001, 1 / 65536)])
+def test_dropout_mask_is_the_definition(ad, rows, cols, p, dtype):
+    """of ones: 0 exactly where the definition drops, the rounded factor everywhere else"""
+    f = ref.keep_factor(rows, cols, p, 3, 4)
+    y = ad.dropout(torch.ones(rows, cols, dtype=dtype, device="cuda"), p, 3, 4)
+    assert torch.equal(y.cpu() != 0, f != 0) and torch.equal(y.cpu(), f.float().to(dtype))
+    res = torch.full((rows, cols), 0.5, dtype=dtype, device="cuda")
+    assert torch.equal(ad.dropout(torch.ones_like(res), p, 3, 4, residual=res).cpu(), (f.float() + 0.5).to(dtype))
+
+
+@pytest.mark.parametrize("rows,e,k,idle", [(70000, 5, 1, 0.0), (20000, 16, 2, 0.4), (16411, 128, 8, 0.1), (300007, 24, 1, 0.2)])
+def test_balance_loss_counts_every_row(ad, rows, e, k, idle):
+    """the longest chain of 32-bit sums is a row, the rows of a lane, the lanes of a wave and the waves of a workgroup: a loss of one valid row more or less is outside"""
+    gen = torch.Generator().manual_seed(rows)
+    logits = 2 * torch.randn(rows, e, generator=gen) + torch.randn(e, generator=gen)
+    ids = logits.topk(k, dim=1).indices
+    mask = torch.rand(rows, generator=gen) >= idle if idle else None
+    want = ref.Balance(logits, ids, mask)
+    lanes = 1
+    while lanes * 8 < e and lanes < 64:
+        lanes *= 2
+    groups = min(256, -(-rows * lanes // 1024))
+    of_a_lane = -(-(-(-rows // groups)) * lanes // 1024)
+    spread = float((logits.max(dim=1).values - logits.min(dim=1).values).max())      # half a step of it in exp's argument
+    # exp: 3 units; the sum of a row, its quotient and product; the rows of a lane; the lanes of a wave and the waves; the result
+    bound = (spread / 2 + 3 + e + 2 + of_a_lane + 6 + 16 + 2) * 2.0 ** -23 * float(want.loss)
+    assert bound < 0.9 * 2 / rows * float(want.loss) or rows > 100000 or e > 100
+    loss, _ = ad.router_balance(logits.cuda(), ids.cuda(), None if mask is None else mask.cuda())
+    assert abs(float(loss) - float(want.loss)) <= bound
