@@ -10,11 +10,12 @@
 // h and dh are held in 32 bits.  In front of 16-bit instructions they are split into three parts of the weights' type, which hold all 24 bits between
 // them: the instructions are not the bound.
 //
-// Measured beside the bytes that a product cannot do without (a copy of the same size moves 5.2 TB/s):
-//   8192 rows, 4096 -> 4096, rank 16, bf16, dropout: shrink 22 us (64 MB, 3.0 TB/s: the generator's products are half of it; without dropout 18, 3.8 TB/s), expand 32 us
-//     (128 MB, 4.2 TB/s), dx 26 us (64 MB and the generator again), outer 31 us (128 MB, 4.3 TB/s), the sum of its chunks 4 us, plan and layout 11 us (latency)
-//   6007 rows, 4096 -> 4096, rank 64, bf16: shrink 18.5 us, expand 28.6 us (98 MB, 3.4 TB/s: 0.3 GB of weights from the L2 beside them), plan and layout 10.5 us
-//   300000 rows, 64 -> 64, rank 8, 32 bits: both products 53.5 us forward (230 MB, 4.3 TB/s), 43 backward (154 MB, 3.6 TB/s), outer 44 us (173 MB, 3.9 TB/s), sum 5.7 us
+// Measured beside the bytes that a product cannot do without (a copy of 1 GiB moves 5.2 TB/s):
+//   8192 rows, 4096 -> 4096, rank 16, bf16, dropout: shrink 22 us (64 MB, 3.0 TB/s: the generator's products are half of it; without dropout 18, 3.8 TB/s), expand 33 us
+//     (128 MB, 4.1 TB/s), dx 27 us (64 MB and the generator again), outer 32 us (128 MB, 4.2 TB/s), the sum of its chunks 4 us, plan and layout 11 to 12 us (latency)
+//   6007 rows, 4096 -> 4096, rank 64, bf16: shrink 18.5 us (47 MB, and 0.13 GB of A from the L2: its ranges are 24 rows), expand 28.9 us (98 MB, 3.4 TB/s, and 0.12 GB of B from the L2), plan and
+//     layout 10.5 us
+//   300000 rows, 64 -> 64, rank 8, 32 bits: both products 53 us forward (230 MB, 4.3 TB/s), 43 backward (154 MB, 3.6 TB/s), outer 45 us (173 MB, 3.8 TB/s), sum 5.3 us
 #pragma once
 #include <type_traits>
 
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(512) lowrank_shrink_kernel(ShrinkArgs q) {
 
 // ---- expand: y[row][n] = base[row][n] + sum_j H[place][j] W[g][n][j] -------------------------------------------------------------------------
 // A wave takes 64 columns of 16, 32 or 64 rows (the weights come from the L2 once for all of them; ranks above 32 stop at 32 rows, whose h leaves room for
-// more waves: rank 64, 6007 rows of 8 KB 28.6 us against 32.6 with 64 rows).  Loads of the next columns are on their way while the last are stored.  The instruction's rows are columns of y in the order that leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of
+// more waves: rank 64, 6007 rows of 8 KB 28.9 us against 32.6 with 64 rows).  Loads of the next columns are on their way while the last are stored.  The instruction's rows are columns of y in the order that leaves a lane pieces of 16 neighbouring bytes, four lanes 64 of
 // them; lanes of rows c and c + 8 then change pieces, so that an access covers 128 bytes of each of 8 rows instead of 64 of 16 (30 against 34 us for
 // a plain copy of 8192 rows of 8 KB in this manner).
 struct ExpandArgs {

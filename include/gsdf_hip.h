@@ -707,11 +707,12 @@ int gsdf_dropout(int64_t rows, int64_t cols, int dtype, const void *x, int64_t x
 
 /* L1  y_t = base_t + s_g B_g A_g drop(x_t) with the adapter g = ids[t] of row t; a row whose id is outside [0, n_adapters) has none and keeps base_t.
  * x [rows, n_in], a [n_adapters, rank, n_in], b [n_adapters, n_out, rank] (contiguous), ids [rows] int32 (ids_64 = 0) or int64, scales [n_adapters] fp32
- * (NULL: 1), base / y [rows, n_out] (base NULL: 0; y may be base, and shares no memory with x).  n_adapters * (rank, as the next of 16, 32, 64 and 128) *
+ * (NULL: 1), base / y [rows, n_out] (base NULL: 0; y may be base, and shares no memory with anything else that the call reads).  n_adapters * (rank, as the next of 16, 32, 64 and 128) *
  * (2 n_in + n_out) is below 2^32.  Dropout as in gsdf_dropout on the matrix x (p = 0: none).
  * fwd: save (gsdf_lowrank_save_bytes) is written for the backward pass, NULL where none follows; ws: gsdf_lowrank_fwd_ws_bytes.
  * bwd: dx [rows, n_in], da, db (any may be NULL) are overwritten, an adapter without rows gets zeros, a row without an adapter dx = 0; dbase = dy is the
- *      caller's.  args, x, ids, a, b and *offset_dev as in the forward call; ws: gsdf_lowrank_bwd_ws_bytes. */
+ *      caller's.  args, x, ids, a, b and *offset_dev as in the forward call; ws: gsdf_lowrank_bwd_ws_bytes.  da and db of rows * (n_in + n_out) above about
+ *      2^39 elements (2^40 of 16 bits) are refused: only rows that lie on one another are so many. */
 #define GSDF_LOWRANK_MAX_RANK 128
 #define GSDF_LOWRANK_MAX_ADAPTERS 1024
 typedef struct {
